@@ -32,6 +32,8 @@ CDF_RENORM = 1
 ATTN_OPS_BF16 = 1
 ATTN_ROWS = 2
 ATTN_XCD_ROWS = 4
+ROPE_INTERLEAVED, ROPE_INVERSE = 1, 2
+EDEV_POS, EDEV_PAGE = 1, 8  # device error word: position, page id
 KV_TILE = 64
 KV_F32, KV_BF16, KV_BF16_NATURAL = 0, 1, 2  # AltxsStepDesc.kv_bf16 / AltxsAttnArgs.kv_bf16
 STEP_SCRATCH_BYTES = 24 << 20  # ALTXS_STEP_SCRATCH_BYTES
@@ -68,6 +70,10 @@ EXPORTS = (
     "altxs_codec_decode",
     "altxs_pack_dense",
     "altxs_pack_dense32",
+    "altxs_rope",
+    "altxs_paged_append",
+    "altxs_paged_attn",
+    "altxs_paged_attn_workspace_bytes",
 )
 
 
@@ -101,6 +107,35 @@ class FfnStageArgs(ctypes.Structure):
                 ("out_w", QTensor), ("up_w", QTensor), ("down_w", QTensor)] + [
                     (n, ctypes.c_void_p) for n in ("y", "hid", "a_sc", "xin", "attn_s", "src", "ln", "scr",
                                                    "m_sc", "x", "lane0", "lane1", "pr", "pp", "skips")]
+
+
+def _fields(**kinds) -> list:
+    """Structure fields in order from runs of names of one C type."""
+    return [(n, t) for names, t in kinds.values() for n in names.split()]
+
+
+class RopeArgs(ctypes.Structure):
+    """AltxsRopeArgs (include/altxs.h)."""
+    _fields_ = _fields(p=("x out pos cos sin err", ctypes.c_void_p),
+                       i64=("T rows x_tok x_head out_tok out_head", ctypes.c_int64),
+                       i32=("H head_dim rot dtype flags reserved", ctypes.c_int32))
+
+
+class PagedAppendArgs(ctypes.Structure):
+    """AltxsPagedAppendArgs (include/altxs.h)."""
+    _fields_ = _fields(p=("k v q q_out k_cache v_cache table pos cu cos sin err", ctypes.c_void_p),
+                       i64=("T n_pages rope_rows k_tok k_head v_tok v_head q_tok q_head q_out_tok q_out_head "
+                            "kc_page kc_head kc_slot vc_page vc_head vc_slot", ctypes.c_int64),
+                       i32=("B H Hkv head_dim page_size table_width rot dtype flags reserved", ctypes.c_int32))
+
+
+class PagedAttnArgs(ctypes.Structure):
+    """AltxsPagedAttnArgs (include/altxs.h)."""
+    _fields_ = _fields(p=("q k_cache v_cache out table pos cu starts prefix slopes err ws", ctypes.c_void_p),
+                       i64=("ws_bytes T n_pages q_tok q_head out_tok out_head "
+                            "kc_page kc_head kc_slot vc_page vc_head vc_slot", ctypes.c_int64),
+                       f32=("scale softcap", ctypes.c_float),
+                       i32=("B H Hkv head_dim page_size table_width max_len window dtype reserved", ctypes.c_int32))
 
 
 class Layer(ctypes.Structure):
@@ -227,6 +262,13 @@ def load():
     L.altxs_pack_dense.argtypes = [p, p, i64, i64, i64, p, p]
     L.altxs_pack_dense32.restype = i32
     L.altxs_pack_dense32.argtypes = [p, p, i64, i64, i64, p, i64, p]
+    for name, args in (("altxs_rope", RopeArgs), ("altxs_paged_append", PagedAppendArgs),
+                       ("altxs_paged_attn", PagedAttnArgs)):
+        f = getattr(L, name)
+        f.restype = i32
+        f.argtypes = [ctypes.POINTER(args), p]
+    L.altxs_paged_attn_workspace_bytes.restype = i64
+    L.altxs_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttnArgs)]
     v = L.altxs_abi_version()
     if v != ABI_VERSION:
         raise AltxsLibraryError(f"{path}: ABI version {v} != {ABI_VERSION}")

@@ -22,7 +22,7 @@ CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libaltxs_hip.so")
 BUILD_DIR = os.path.join(ROOT, "_build", "altxs_hip")
 SOURCES = ("api.cpp", "cdf.hip", "qgemm.hip", "qgemv.hip", "stages.hip", "attn.hip", "step.hip", "persist.hip",
-           "coder.hip", "codec.hip")
+           "coder.hip", "codec.hip", "rope.hip", "paged_attn.hip")
 ARCH = os.environ.get("ALTXS_ARCH", "gfx950")
 
 

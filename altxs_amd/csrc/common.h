@@ -140,6 +140,7 @@ enum : int32_t {
   ALTXS_EDEV_POS = 1,    // position >= max_len (KV write/read skipped)
   ALTXS_EDEV_TOKEN = 2,  // token id outside [0, V) (clamped)
   ALTXS_EDEV_SPIN = 4,   // a persistent-kernel wait gave up (results invalid, kernel exited)
+  ALTXS_EDEV_PAGE = 8,   // page id outside the pool (row skipped)
 };
 __device__ __forceinline__ void flag_err(int32_t* err, int32_t code) {
   if (err) atomicOr(err, code);

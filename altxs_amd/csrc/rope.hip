@@ -1,0 +1,350 @@
+// Rotary positions, alone (altxs_rope) and on the way into a paged KV cache
+// (altxs_paged_append).  (a, b) -> (a cos + b sin, b cos - a sin) for each pair
+// of a head's first `rot` dims, the sign of the step's QKV epilogue
+// (apply_rotary_emb, src/xsa_ttt/model.py:195-206).
+//
+// Both only move data (3 flops per element), so they are built to read and write
+// every element once in 16-byte accesses: a head's row is cut into units -- one
+// 16-byte vector of first and one of second elements (half layout), one vector
+// of whole pairs (interleaved), or one vector of unrotated dims -- and a
+// workgroup takes whole tokens, consecutive threads consecutive units.  Rows
+// that 16-byte accesses do not fit (strides, alignment, rot) go by units of one
+// pair or one element.
+#include <type_traits>
+
+#include "common.h"
+#include "paged.h"
+
+namespace {
+
+using namespace altxs_paged;
+
+constexpr int THREADS = 256;
+
+template <class T> struct alignas(16) Vec { T v[16 / sizeof(T)]; };
+
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(__bf16 x) { return (float)x; }
+__device__ __forceinline__ float to_f(_Float16 x) { return (float)x; }
+
+// How a head's row is cut into units.
+struct Units {
+  int nrot;   // rotated units
+  int total;  // nrot + units of unrotated dims
+  int half;   // rot / 2
+};
+
+// One unit of one head row.  cs/sn: the position's table rows (NULL: copy).
+template <class T, bool VEC, bool INTER>
+__device__ __forceinline__ void move_unit(const T* src, T* dst, const float* cs, const float* sn, float sgn,
+                                          const Units u, int i) {
+#pragma clang fp contract(off)
+  constexpr int N = VEC ? 16 / (int)sizeof(T) : 1;
+  if (i >= u.nrot) {  // unrotated dims
+    const int d = 2 * u.half + (i - u.nrot) * N;
+    if constexpr (VEC) *(Vec<T>*)(dst + d) = *(const Vec<T>*)(src + d);
+    else dst[d] = src[d];
+    return;
+  }
+  if constexpr (VEC && INTER) {
+    const int d = i * N;
+    Vec<T> x = *(const Vec<T>*)(src + d);
+    if (cs) {
+      typedef __attribute__((ext_vector_type(N / 2))) float pairs_t;
+      const pairs_t c = *(const pairs_t*)(cs + d / 2), s = sgn * *(const pairs_t*)(sn + d / 2);
+#pragma unroll
+      for (int j = 0; j < N / 2; ++j) {
+        const float a = to_f(x.v[2 * j]), b = to_f(x.v[2 * j + 1]);
+        x.v[2 * j] = (T)__builtin_fmaf(b, s[j], a * c[j]);
+        x.v[2 * j + 1] = (T)__builtin_fmaf(-a, s[j], b * c[j]);
+      }
+    }
+    *(Vec<T>*)(dst + d) = x;
+  } else if constexpr (VEC) {
+    const int d = i * N;
+    Vec<T> x = *(const Vec<T>*)(src + d), y = *(const Vec<T>*)(src + u.half + d);
+    if (cs) {
+      float c[N], s[N];
+#pragma unroll
+      for (int j = 0; j < N; j += 4) {
+        *(f32x4*)(c + j) = *(const f32x4*)(cs + d + j);
+        *(f32x4*)(s + j) = *(const f32x4*)(sn + d + j);
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float a = to_f(x.v[j]), b = to_f(y.v[j]), sj = sgn * s[j];
+        x.v[j] = (T)__builtin_fmaf(b, sj, a * c[j]);
+        y.v[j] = (T)__builtin_fmaf(-a, sj, b * c[j]);
+      }
+    }
+    *(Vec<T>*)(dst + d) = x;
+    *(Vec<T>*)(dst + u.half + d) = y;
+  } else {
+    const int d0 = INTER ? 2 * i : i, d1 = INTER ? d0 + 1 : i + u.half;
+    const float a = to_f(src[d0]), b = to_f(src[d1]);
+    if (cs) {
+      const float c = cs[i], s = sgn * sn[i];
+      dst[d0] = (T)__builtin_fmaf(b, s, a * c);
+      dst[d1] = (T)__builtin_fmaf(-a, s, b * c);
+    } else {
+      dst[d0] = (T)a;
+      dst[d1] = (T)b;
+    }
+  }
+}
+
+struct RopeP {
+  const void* x;
+  void* out;
+  const int32_t* pos;
+  const float *cos, *sin;
+  int32_t* err;
+  int64_t T, rows, x_tok, x_head, out_tok, out_head;
+  Units u;
+  FastDiv by_units;  // units of a head
+  FastDiv by_token;  // units of a token
+  int tpb;           // tokens of a workgroup
+  float sgn;
+};
+
+template <class T, bool VEC, bool INTER>
+__global__ __launch_bounds__(THREADS) void rope_kernel(RopeP p) {
+  const int64_t t0 = (int64_t)blockIdx.x * p.tpb;
+  const int nt = (int)(p.T - t0 < p.tpb ? p.T - t0 : p.tpb);
+  const int n = nt * (int)p.by_token.d;
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const uint32_t tl = div_by(i, p.by_token), j = i - tl * p.by_token.d;
+    const uint32_t h = div_by(j, p.by_units), u = j - h * p.by_units.d;
+    const int64_t t = t0 + tl;
+    const int32_t pos = p.pos[t];
+    const bool ok = pos >= 0 && pos < p.rows;
+    if (!ok && pos >= 0 && j == 0) flag_err(p.err, ALTXS_EDEV_POS);
+    const float* cs = ok ? p.cos + (int64_t)pos * p.u.half : nullptr;
+    const float* sn = ok ? p.sin + (int64_t)pos * p.u.half : nullptr;
+    move_unit<T, VEC, INTER>((const T*)p.x + t * p.x_tok + h * p.x_head, (T*)p.out + t * p.out_tok + h * p.out_head, cs, sn,
+                             p.sgn, p.u, u);
+  }
+}
+
+struct AppendP {
+  const void *k, *v, *q;
+  void *q_out, *k_cache, *v_cache;
+  const int32_t *table, *pos, *cu;
+  const float *cos, *sin;
+  int32_t* err;
+  int64_t T, n_pages, rope_rows;
+  int64_t k_tok, k_head, v_tok, v_head, q_tok, q_head, qo_tok, qo_head;
+  int64_t kc_page, kc_head, kc_slot, vc_page, vc_head, vc_slot;
+  int B, Hq, Hkv, width, shift, W;  // Hq: query heads moved here (0: none); W: tokens of a segment (cu = NULL)
+  Units u;
+  FastDiv by_units, by_token;
+  int tpb;
+};
+
+// A token's place: its rope row and its cache row's element offsets (ok = 0: skipped).
+struct Place {
+  int64_t koff, voff;
+  int32_t pos, ok;
+};
+
+constexpr int MAX_TPB = 64;
+
+// The workgroup's tokens find their segments first, a wave per token: the number
+// of entries cu[1..B] at or below the token, 64 of them per step.
+template <class T, bool VEC, bool INTER>
+__global__ __launch_bounds__(THREADS) void append_kernel(AppendP p) {
+  __shared__ Place place[MAX_TPB];
+  const int64_t t0 = (int64_t)blockIdx.x * p.tpb;
+  const int nt = (int)(p.T - t0 < p.tpb ? p.T - t0 : p.tpb);
+  const int wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE;
+  for (int tl = wave; tl < nt; tl += THREADS / WAVE) {
+    const int64_t t = t0 + tl;
+    int b, c0, c1;
+    if (p.cu) {
+      b = 0;
+      for (int i = 0; i < p.B; i += WAVE)
+        b += __builtin_popcountll(__ballot(i + lane < p.B && p.cu[i + lane + 1] <= t));
+      c0 = b < p.B ? p.cu[b] : 0;
+      c1 = b < p.B ? p.cu[b + 1] : 0;
+    } else {
+      b = (int)(t / p.W);
+      c0 = b * p.W;
+      c1 = c0 + p.W;
+    }
+    if (lane == 0) {
+      Place pl = {0, 0, 0, 0};
+      if (b < p.B) {  // rows behind the last segment belong to nobody
+        const int64_t cap = (int64_t)p.width << p.shift;
+        const Segment s = segment_of(c0, c1, p.pos[b], p.T, (int32_t)(cap < INT32_MAX ? cap : INT32_MAX));
+        const int32_t pos = s.pos + (int32_t)(t - s.t0);
+        if (!s.ok || t < s.t0 || t >= s.t0 + s.n || (p.cos && pos >= p.rope_rows)) {
+          flag_err(p.err, ALTXS_EDEV_POS);
+        } else {
+          const int32_t g = page_of(p.table + (int64_t)b * p.width, p.width, p.shift, p.n_pages, pos);
+          if (g < 0) {
+            flag_err(p.err, ALTXS_EDEV_PAGE);
+          } else {
+            const int slot = pos & ((1 << p.shift) - 1);
+            pl.koff = g * p.kc_page + slot * p.kc_slot;
+            pl.voff = g * p.vc_page + slot * p.vc_slot;
+            pl.ok = 1;
+          }
+          pl.pos = pos;
+        }
+      }
+      place[tl] = pl;
+    }
+  }
+  __syncthreads();
+  const int n = nt * (int)p.by_token.d;
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const uint32_t tl = div_by(i, p.by_token), j = i - tl * p.by_token.d;
+    int h = (int)div_by(j, p.by_units);
+    const int u = (int)(j - h * p.by_units.d);
+    const Place pl = place[tl];
+    if (!pl.ok) continue;
+    const int64_t t = t0 + tl;
+    const float* cs = p.cos ? p.cos + (int64_t)pl.pos * p.u.half : nullptr;
+    const float* sn = p.cos ? p.sin + (int64_t)pl.pos * p.u.half : nullptr;
+    const T* src;
+    T* dst;
+    if (h < p.Hq) {
+      src = (const T*)p.q + t * p.q_tok + h * p.q_head;
+      dst = (T*)p.q_out + t * p.qo_tok + h * p.qo_head;
+    } else if ((h -= p.Hq) < p.Hkv) {
+      src = (const T*)p.k + t * p.k_tok + h * p.k_head;
+      dst = (T*)p.k_cache + pl.koff + h * p.kc_head;
+    } else {
+      h -= p.Hkv;
+      src = (const T*)p.v + t * p.v_tok + h * p.v_head;
+      dst = (T*)p.v_cache + pl.voff + h * p.vc_head;
+      cs = nullptr;
+    }
+    move_unit<T, VEC, INTER>(src, dst, cs, sn, 1.f, p.u, u);
+  }
+}
+
+int elem_size(int dtype) { return dtype == ALTXS_F32 ? 4 : 2; }
+
+// Whether rows with these strides (in elements) at p can be moved in 16-byte vectors.
+bool fits16(const void* p, int n, std::initializer_list<int64_t> strides) {
+  bool ok = ((uintptr_t)p & 15) == 0;
+  for (int64_t s : strides) ok = ok && s % n == 0;
+  return ok;
+}
+
+// Vectors need whole ones in the head, the unrotated dims and each half (pairs).
+bool dims_fit(int hd, int rot, bool inter, int n) { return hd % n == 0 && (inter ? rot % n == 0 : rot % (2 * n) == 0); }
+
+Units units_of(int hd, int rot, bool vec, bool inter, int n) {
+  Units u;
+  u.half = rot / 2;
+  if (!vec) n = 1;
+  u.nrot = vec ? (inter ? rot / n : rot / 2 / n) : rot / 2;
+  u.total = u.nrot + (hd - rot) / n;
+  return u;
+}
+
+#define BY_TYPE(KERNEL, dtype, vec, inter, grid, s, p)                                                    \
+  do {                                                                                                    \
+    auto go = [&](auto t) {                                                                               \
+      using T = decltype(t);                                                                              \
+      if (vec && inter) hipLaunchKernelGGL((KERNEL<T, true, true>), grid, dim3(THREADS), 0, s, p);        \
+      else if (vec) hipLaunchKernelGGL((KERNEL<T, true, false>), grid, dim3(THREADS), 0, s, p);           \
+      else if (inter) hipLaunchKernelGGL((KERNEL<T, false, true>), grid, dim3(THREADS), 0, s, p);         \
+      else hipLaunchKernelGGL((KERNEL<T, false, false>), grid, dim3(THREADS), 0, s, p);                   \
+    };                                                                                                    \
+    if (dtype == ALTXS_F32) go(float{});                                                                  \
+    else if (dtype == ALTXS_BF16) go(__bf16{});                                                           \
+    else go(_Float16{});                                                                                  \
+  } while (0)
+
+}  // namespace
+
+extern "C" int32_t altxs_rope(const AltxsRopeArgs* a, altxs_stream_t stream) {
+  ALTXS_REQUIRE(a, "altxs_rope: null pointer");
+  ALTXS_REQUIRE(a->dtype == ALTXS_F32 || a->dtype == ALTXS_BF16 || a->dtype == ALTXS_F16,
+                "altxs_rope: dtype=%d", a->dtype);
+  ALTXS_REQUIRE((a->flags & ~(ALTXS_ROPE_INTERLEAVED | ALTXS_ROPE_INVERSE)) == 0, "altxs_rope: unknown flags 0x%x",
+                a->flags);
+  ALTXS_REQUIRE(a->head_dim >= 2 && a->head_dim <= 1024, "altxs_rope: head_dim=%d", a->head_dim);
+  ALTXS_REQUIRE(a->rot >= 2 && a->rot % 2 == 0 && a->rot <= a->head_dim,
+                "altxs_rope: rot=%d must be even, 2 to head_dim=%d", a->rot, a->head_dim);
+  ALTXS_REQUIRE(a->H >= 1 && a->H <= 4096, "altxs_rope: H=%d", a->H);
+  ALTXS_REQUIRE(a->T >= 0 && a->rows >= 1, "altxs_rope: bad T or rows");
+  if (a->T == 0) return ALTXS_OK;
+  ALTXS_REQUIRE(a->x && a->out && a->pos && a->cos && a->sin, "altxs_rope: null pointer");
+  const int n = 16 / elem_size(a->dtype);
+  const bool inter = (a->flags & ALTXS_ROPE_INTERLEAVED) != 0;
+  const bool vec = dims_fit(a->head_dim, a->rot, inter, n) && fits16(a->x, n, {a->x_tok, a->x_head}) &&
+                   fits16(a->out, n, {a->out_tok, a->out_head}) && fits16(a->cos, 4, {(int64_t)a->rot / 2}) &&
+                   fits16(a->sin, 4, {(int64_t)a->rot / 2});
+  RopeP p;
+  p.x = a->x; p.out = a->out; p.pos = a->pos; p.cos = a->cos; p.sin = a->sin; p.err = a->err;
+  p.T = a->T; p.rows = a->rows;
+  p.x_tok = a->x_tok; p.x_head = a->x_head; p.out_tok = a->out_tok; p.out_head = a->out_head;
+  p.u = units_of(a->head_dim, a->rot, vec, inter, n);
+  p.sgn = a->flags & ALTXS_ROPE_INVERSE ? -1.f : 1.f;
+  if (a->x == a->out && a->x_tok == a->out_tok && a->x_head == a->out_head) p.u.total = p.u.nrot;  // the rest stays
+  p.by_units = fast_div(p.u.total);
+  p.by_token = fast_div(p.u.total * a->H);
+  p.tpb = (int)p.by_token.d >= THREADS ? 1 : THREADS / (int)p.by_token.d;
+  const int64_t wgs = (a->T + p.tpb - 1) / p.tpb;
+  ALTXS_REQUIRE(wgs < (1ll << 31), "altxs_rope: T=%lld", (long long)a->T);
+  const dim3 grid((unsigned)wgs);
+  BY_TYPE(rope_kernel, a->dtype, vec, inter, grid, (hipStream_t)stream, p);
+  ALTXS_CHECK_HIP(hipGetLastError());
+  return ALTXS_OK;
+}
+
+extern "C" int32_t altxs_paged_append(const AltxsPagedAppendArgs* a, altxs_stream_t stream) {
+  ALTXS_REQUIRE(a, "altxs_paged_append: null pointer");
+  ALTXS_REQUIRE(a->dtype == ALTXS_F32 || a->dtype == ALTXS_BF16 || a->dtype == ALTXS_F16,
+                "altxs_paged_append: dtype=%d", a->dtype);
+  ALTXS_REQUIRE((a->flags & ~ALTXS_ROPE_INTERLEAVED) == 0, "altxs_paged_append: unknown flags 0x%x", a->flags);
+  ALTXS_REQUIRE(a->head_dim >= 2 && a->head_dim <= 1024, "altxs_paged_append: head_dim=%d", a->head_dim);
+  ALTXS_REQUIRE(a->rot >= 0 && a->rot % 2 == 0 && a->rot <= a->head_dim,
+                "altxs_paged_append: rot=%d must be even, 0 to head_dim=%d", a->rot, a->head_dim);
+  ALTXS_REQUIRE(a->Hkv >= 1 && a->Hkv <= 4096 && (!a->q || (a->H >= 1 && a->H <= 4096)), "altxs_paged_append: H=%d Hkv=%d",
+                a->H, a->Hkv);
+  ALTXS_REQUIRE(a->page_size >= 16 && a->page_size <= 1024 && (a->page_size & (a->page_size - 1)) == 0,
+                "altxs_paged_append: page_size=%d must be a power of two from 16 to 1024", a->page_size);
+  ALTXS_REQUIRE(a->T >= 0 && a->T < (1ll << 31) && a->B >= 0 && a->n_pages >= 0 && a->table_width >= 0,
+                "altxs_paged_append: bad T, B, n_pages or table_width");
+  ALTXS_REQUIRE(a->rot > 0 || !a->q, "altxs_paged_append: q without a rotation");
+  if (a->T == 0 || a->B == 0) return ALTXS_OK;
+  ALTXS_REQUIRE(a->cu || a->T % a->B == 0, "altxs_paged_append: T=%lld tokens are not B=%d equal segments",
+                (long long)a->T, a->B);
+  ALTXS_REQUIRE(a->k && a->v && a->k_cache && a->v_cache && a->table && a->pos && (!a->q || a->q_out) &&
+                    (a->rot == 0 || (a->cos && a->sin)),
+                "altxs_paged_append: null pointer");
+  ALTXS_REQUIRE(a->rot == 0 || a->rope_rows >= 1, "altxs_paged_append: rope_rows=%lld", (long long)a->rope_rows);
+  const int n = 16 / elem_size(a->dtype);
+  const bool inter = (a->flags & ALTXS_ROPE_INTERLEAVED) != 0;
+  bool vec = dims_fit(a->head_dim, a->rot, inter, n) && fits16(a->k, n, {a->k_tok, a->k_head}) &&
+             fits16(a->v, n, {a->v_tok, a->v_head}) && fits16(a->k_cache, n, {a->kc_page, a->kc_head, a->kc_slot}) &&
+             fits16(a->v_cache, n, {a->vc_page, a->vc_head, a->vc_slot});
+  if (a->q) vec = vec && fits16(a->q, n, {a->q_tok, a->q_head}) && fits16(a->q_out, n, {a->q_out_tok, a->q_out_head});
+  if (a->rot) vec = vec && fits16(a->cos, 4, {(int64_t)a->rot / 2}) && fits16(a->sin, 4, {(int64_t)a->rot / 2});
+  AppendP p;
+  p.k = a->k; p.v = a->v; p.q = a->q; p.q_out = a->q_out; p.k_cache = a->k_cache; p.v_cache = a->v_cache;
+  p.table = a->table; p.pos = a->pos; p.cu = a->cu;
+  p.cos = a->rot ? a->cos : nullptr; p.sin = a->sin; p.err = a->err;
+  p.T = a->T; p.n_pages = a->n_pages; p.rope_rows = a->rope_rows;
+  p.k_tok = a->k_tok; p.k_head = a->k_head; p.v_tok = a->v_tok; p.v_head = a->v_head;
+  p.q_tok = a->q_tok; p.q_head = a->q_head; p.qo_tok = a->q_out_tok; p.qo_head = a->q_out_head;
+  p.kc_page = a->kc_page; p.kc_head = a->kc_head; p.kc_slot = a->kc_slot;
+  p.vc_page = a->vc_page; p.vc_head = a->vc_head; p.vc_slot = a->vc_slot;
+  p.B = a->B; p.Hq = a->q ? a->H : 0; p.Hkv = a->Hkv; p.width = a->table_width;
+  p.shift = __builtin_ctz((unsigned)a->page_size);
+  p.W = a->cu ? 1 : (int)(a->T / a->B);
+  p.u = units_of(a->head_dim, a->rot, vec, inter, n);
+  p.by_units = fast_div(p.u.total);
+  p.by_token = fast_div(p.u.total * (p.Hq + 2 * p.Hkv));
+  p.tpb = (int)p.by_token.d >= THREADS ? 1 : THREADS / (int)p.by_token.d;
+  if (p.tpb > MAX_TPB) p.tpb = MAX_TPB;
+  const dim3 grid((unsigned)((a->T + p.tpb - 1) / p.tpb));
+  BY_TYPE(append_kernel, a->dtype, vec, inter, grid, (hipStream_t)stream, p);
+  ALTXS_CHECK_HIP(hipGetLastError());
+  return ALTXS_OK;
+}

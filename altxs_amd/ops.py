@@ -11,6 +11,14 @@ replace:
 * :func:`dequant`       <- ``dequantize_channels`` (mixed_bit_delta.py:172-229);
 * :func:`qgemm`         <- ``gemv_rows(x, w, out)`` (src/xsa_ttt/ac_gemv.py:391-420);
 * :func:`decode_attn`   <- ``run_split_attn`` (src/xsa_ttt/split_attn.py:341-425).
+
+Serving from a paged KV cache (:mod:`altxs_amd.paged` holds the cache itself):
+
+* :func:`rope`, :func:`rope_tables` -- rotary positions
+  (``apply_rotary_emb`` / ``Rotary``, src/xsa_ttt/model.py:130-206) of any head
+  layout, and their tables for long contexts;
+* :func:`paged_append` -- new keys and values into their pages, rotated on the way;
+* :func:`paged_attn` -- attention of one or more new tokens per segment over the pages.
 """
 
 from __future__ import annotations
@@ -198,3 +206,276 @@ def decode_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pos: torch.Te
     rc = _lib.load().altxs_decode_attn(ctypes.byref(a), _s(q))
     _lib.check(rc, "altxs_decode_attn")
     return y
+
+
+# ---- serving from a paged KV cache -------------------------------------------
+
+
+def rope_tables(length: int, rot: int, base: float = 1e4, *, scaling: str | None = None, factor: float = 1.0,
+                trained_len: int = 2048, device="cuda"):
+    """cos/sin fp32 [length, rot/2] of the rotary angles pos * base^(-2i/rot).
+
+    The angles are formed in float64, so far positions keep theirs (position 10^6
+    in fp32 would be off by 0.03 rad).  ``scaling`` stretches them for contexts
+    ``factor`` times the ``trained_len`` tokens a model was trained on:
+
+    * ``"linear"``: positions divided by the factor;
+    * ``"ntk"``: base * factor^(rot/(rot-2)), the rule of the reference's Rotary
+      (src/xsa_ttt/model.py:147-192);
+    * ``"yarn"``: dims that turn more than 32 times in ``trained_len`` tokens stay,
+      those that turn less than once are divided by the factor, a linear ramp
+      between, and cos/sin carry the method's 0.1 ln(factor) + 1 (arXiv 2309.00071).
+    """
+    if rot < 2 or rot % 2 or length < 1:
+        raise ValueError(f"rope_tables: rot={rot} must be even and length={length} positive")
+    if scaling not in (None, "linear", "ntk", "yarn") or factor < 1.0:
+        raise ValueError(f"rope_tables: scaling={scaling!r} factor={factor}")
+    if scaling == "ntk":
+        if rot == 2:
+            raise ValueError("rope_tables: ntk scaling needs rot > 2")
+        base = base * factor ** (rot / (rot - 2))
+    freq = base ** -(np.arange(0, rot, 2, dtype=np.float64) / rot)
+    mag = 1.0
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "yarn":
+        turns = freq * trained_len / (2 * np.pi)
+        keep = np.clip((turns - 1.0) / 31.0, 0.0, 1.0)
+        freq = freq * keep + freq / factor * (1.0 - keep)
+        mag = 0.1 * np.log(factor) + 1.0
+    ang = np.outer(np.arange(length, dtype=np.float64), freq)
+    return tuple(torch.from_numpy((mag * f(ang)).astype(np.float32)).to(device) for f in (np.cos, np.sin))
+
+
+def _heads(t: torch.Tensor, name: str, like: torch.Tensor | None = None) -> None:
+    """A [T, heads, head_dim] device tensor whose heads are contiguous."""
+    if t.dim() != 3 or not t.is_cuda or t.stride(2) != 1:
+        raise ValueError(f"{name} must be a device tensor [T, heads, head_dim] with contiguous heads")
+    if t.dtype not in _DT:
+        raise ValueError(f"{name} dtype {t.dtype} not supported")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise ValueError(f"{name} must have the dtype and device of the other heads")
+
+
+def _written(t: torch.Tensor, name: str, *reads: torch.Tensor) -> None:
+    """An output every element of which is its own, apart from or equal to what is read."""
+    for n, st in zip(t.shape, t.stride()):
+        if n > 1 and st == 0:
+            raise ValueError(f"{name} must not be expanded")
+    for x in reads:
+        if x.data_ptr() == t.data_ptr() and x.stride() == t.stride():
+            continue
+        lo, hi = t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+        xl = x.data_ptr()
+        xh = xl + x.element_size() * (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride())))
+        if x.numel() and t.numel() and lo < xh and xl < hi:
+            raise ValueError(f"{name} must be the input itself or not overlap it")
+
+
+def _index(t: torch.Tensor, name: str, n: int, dev) -> int:
+    if t.dtype != torch.int32 or t.device != dev or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor [{n}] on {dev}")
+    return t.data_ptr()
+
+
+def _err(err: torch.Tensor | None, dev):
+    if err is None:
+        return None
+    if err.dtype != torch.int32 or err.device != dev or err.numel() < 1:
+        raise ValueError(f"err must be an int32 tensor on {dev}")
+    return err.data_ptr()
+
+
+def _rot_tables(cos: torch.Tensor, sin: torch.Tensor, hd: int, dev) -> int:
+    """rot of a pair of tables [rows, rot/2]."""
+    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape != sin.shape
+            or cos.device != dev or sin.device != dev or not cos.is_contiguous() or not sin.is_contiguous()):
+        raise ValueError(f"cos and sin must be contiguous fp32 tensors [rows, rot/2] on {dev}")
+    rot = 2 * cos.shape[1]
+    if not 2 <= rot <= hd or cos.shape[0] < 1:
+        raise ValueError(f"tables of {rot} dims for heads of {hd}")
+    return rot
+
+
+def _launch(name: str, args, dev) -> None:
+    """Call ``name`` on the current stream of ``dev`` (which need not be the current device)."""
+    f = getattr(_lib.load(), name)
+    if dev.index == torch.cuda.current_device():
+        rc = f(ctypes.byref(args), torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = f(ctypes.byref(args), torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        _lib.check(rc, name)
+
+
+def rope(x: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *, interleaved: bool = False,
+         inverse: bool = False, out: torch.Tensor | None = None, err: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions: x [T, H, hd] (fp32, bf16 or fp16, any token and head
+    strides), pos [T] int32, cos/sin fp32 [rows, rot/2].
+
+    The pairs (a, b) of each head's first ``rot`` dims -- (i, i + rot/2), or
+    (2i, 2i + 1) with ``interleaved`` -- become (a cos + b sin, b cos - a sin), the
+    reference's sign (src/xsa_ttt/model.py:195-206); ``inverse`` turns the other
+    way, which is also the gradient.  ``out`` may be ``x``.  Rows whose position is
+    outside the tables are copied unrotated and, unless it is negative
+    (padding), flagged in ``err`` (int32).
+    """
+    _heads(x, "x")
+    T, H, hd = x.shape
+    dev = x.device
+    rot = _rot_tables(cos, sin, hd, dev)
+    if out is None:
+        out = torch.empty(T, H, hd, dtype=x.dtype, device=dev)
+    else:
+        _heads(out, "out", x)
+        if out.shape != x.shape:
+            raise ValueError(f"out must have x's shape {tuple(x.shape)}")
+        _written(out, "out", x)
+    a = _lib.RopeArgs(x.data_ptr(), out.data_ptr(), _index(pos, "pos", T, dev), cos.data_ptr(), sin.data_ptr(),
+                      _err(err, dev), T, cos.shape[0], x.stride(0), x.stride(1), out.stride(0), out.stride(1), H, hd, rot,
+                      _DT[x.dtype], (_lib.ROPE_INTERLEAVED if interleaved else 0) | (_lib.ROPE_INVERSE if inverse else 0))
+    if H:
+        _launch("altxs_rope", a, dev)
+    return out
+
+
+def _pages(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, pos: torch.Tensor,
+           cu: torch.Tensor | None, like: torch.Tensor) -> int:
+    """Check the cache's arrays; returns the number of segments."""
+    dev = like.device
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
+        raise ValueError("k_cache and v_cache must be equal [n_pages, Hkv, page_size, head_dim] with contiguous rows")
+    if k_cache.dtype != like.dtype or v_cache.dtype != like.dtype or k_cache.device != dev or v_cache.device != dev:
+        raise ValueError("the caches must have the dtype and device of the heads")
+    if table.dim() != 2 or table.dtype != torch.int32 or table.device != dev or not table.is_contiguous():
+        raise ValueError(f"table must be a contiguous int32 tensor [segments, pages] on {dev}")
+    B = table.shape[0]
+    _index(pos, "pos", B, dev)
+    if cu is not None:
+        _index(cu, "cu", B + 1, dev)
+    elif B and like.shape[0] % B:
+        raise ValueError(f"{like.shape[0]} tokens are not {B} equal segments (give cu)")
+    return B
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor,
+                 pos: torch.Tensor, *, cu: torch.Tensor | None = None, q: torch.Tensor | None = None,
+                 q_out: torch.Tensor | None = None, cos: torch.Tensor | None = None, sin: torch.Tensor | None = None,
+                 interleaved: bool = False, err: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Write new keys and values k, v [T, Hkv, hd] into their segments' pages.
+
+    k_cache/v_cache [n_pages, Hkv, page_size, hd] (any strides, contiguous rows;
+    page_size a power of two, 16 to 1024), table int32 [B, width] (page ids in
+    order), pos int32 [B]: new token t of segment b goes to position pos[b] + t.
+    ``cu`` int32 [B + 1]: segment b's tokens are rows cu[b] to cu[b+1] (default:
+    T / B each); rows from cu[B] on are left alone.  With tables ``cos``/``sin`` the
+    keys are rotated by their positions on the way (as :func:`rope`), and so
+    is ``q`` [T, H, hd] into ``q_out`` (default: a new tensor; may be ``q``), which
+    is returned -- a new one's rows that belong to no segment, or to one that was
+    left out (``err``), are not written.  Without tables ``q`` is returned as it is.
+    """
+    _heads(k, "k")
+    _heads(v, "v", k)
+    T, Hkv, hd = k.shape
+    dev = k.device
+    if v.shape != k.shape:
+        raise ValueError("k and v must have equal shapes")
+    B = _pages(k_cache, v_cache, table, pos, cu, k)
+    n_pages, ch, page, chd = k_cache.shape
+    if ch != Hkv or chd != hd:
+        raise ValueError(f"caches of {ch} heads of {chd}, keys of {Hkv} of {hd}")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin go together")
+    _written(k_cache, "k_cache", k, v)
+    _written(v_cache, "v_cache", k, v)
+    rot, H, qp, qo, qs, os_ = 0, 0, None, None, (0, 0, 0), (0, 0, 0)
+    result = q
+    if cos is not None:
+        rot = _rot_tables(cos, sin, hd, dev)
+        if q is not None:
+            _heads(q, "q", k)
+            if q.shape[0] != T or q.shape[2] != hd:
+                raise ValueError(f"q must be [{T}, heads, {hd}]")
+            result = torch.empty(q.shape, dtype=q.dtype, device=dev) if q_out is None else q_out
+            if q_out is not None:
+                _heads(q_out, "q_out", q)
+                if q_out.shape != q.shape:
+                    raise ValueError(f"q_out must have q's shape {tuple(q.shape)}")
+                _written(q_out, "q_out", q)
+                _written(q_out, "q_out", k, v)
+            H = q.shape[1]
+            if H:
+                qp, qo, qs, os_ = q.data_ptr(), result.data_ptr(), q.stride(), result.stride()
+    elif q_out is not None:
+        raise ValueError("q_out without cos and sin")
+    ks, vs, kc, vc = k.stride(), v.stride(), k_cache.stride(), v_cache.stride()
+    a = _lib.PagedAppendArgs(k.data_ptr(), v.data_ptr(), qp, qo, k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(),
+                             pos.data_ptr(), cu.data_ptr() if cu is not None else None,
+                             cos.data_ptr() if rot else None, sin.data_ptr() if rot else None, _err(err, dev),
+                             T, n_pages, cos.shape[0] if rot else 0, ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], os_[0], os_[1],
+                             kc[0], kc[1], kc[2], vc[0], vc[1], vc[2], B, H, Hkv, hd, page, table.shape[1], rot,
+                             _DT[k.dtype], _lib.ROPE_INTERLEAVED if interleaved and rot else 0)
+    if Hkv:
+        _launch("altxs_paged_append", a, dev)
+    return result
+
+
+def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, pos: torch.Tensor, *,
+               cu: torch.Tensor | None = None, max_len: int | None = None, scale: float | None = None,
+               softcap: float = 0.0, slopes: torch.Tensor | None = None, window: int = 0,
+               starts: torch.Tensor | None = None, prefix: torch.Tensor | None = None,
+               out: torch.Tensor | None = None, err: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of the new tokens q [T, H, hd] (hd 64 or 128) over their segments'
+    pages, in which their own keys and values already are (:func:`paged_append`
+    with the same table, pos and cu); H a multiple of the cache's heads.
+
+    The token at position p sees the keys [lo, hi): hi = p + 1, or the first
+    ``prefix[b]`` keys of the segment if that is more (int32 [B]; a prefix mask);
+    lo = max(0, p - window + 1 (``window`` > 0), ``starts[t]`` (int32 [T], the position
+    where the token's document begins)).  Scores are scale * q.k (default
+    hd^-1/2), then softcap * tanh(. / softcap) if ``softcap`` > 0, then minus
+    ``slopes[h]`` (fp32 [H]) * |p - key|.  A token that sees nothing gets zeros; rows
+    behind the last segment keep what ``out`` held.
+
+    ``max_len``: the most keys any segment has (default: what its table can
+    hold); it sizes the launch, so give it where it is known.  A row's bits
+    depend on the row's own query, keys and masks alone.
+    """
+    _heads(q, "q")
+    T, H, hd = q.shape
+    dev = q.device
+    B = _pages(k_cache, v_cache, table, pos, cu, q)
+    n_pages, Hkv, page, chd = k_cache.shape
+    if chd != hd:
+        raise ValueError(f"caches of heads of {chd}, queries of {hd}")
+    width = table.shape[1]
+    max_len = width * page if max_len is None else int(max_len)
+    if out is None:
+        out = torch.empty(T, H, hd, dtype=q.dtype, device=dev)
+    else:
+        _heads(out, "out", q)
+        if out.shape != q.shape:
+            raise ValueError(f"out must have q's shape {tuple(q.shape)}")
+        _written(out, "out", q)
+        _written(out, "out", k_cache, v_cache)
+    if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (H,) or slopes.device != dev
+                               or not slopes.is_contiguous()):
+        raise ValueError(f"slopes must be a contiguous fp32 tensor [{H}] on {dev}")
+    qs, os_, kc, vc = q.stride(), out.stride(), k_cache.stride(), v_cache.stride()
+    a = _lib.PagedAttnArgs(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), table.data_ptr(),
+                           pos.data_ptr(), cu.data_ptr() if cu is not None else None,
+                           _index(starts, "starts", T, dev) if starts is not None else None,
+                           _index(prefix, "prefix", B, dev) if prefix is not None else None,
+                           slopes.data_ptr() if slopes is not None else None, _err(err, dev), None, 0, T, n_pages,
+                           qs[0], qs[1], os_[0], os_[1], kc[0], kc[1], kc[2], vc[0], vc[1], vc[2],
+                           hd ** -0.5 if scale is None else scale, softcap, B, H, Hkv, hd, page, width, max_len, window,
+                           _DT[q.dtype])
+    n = _lib.load().altxs_paged_attn_workspace_bytes(ctypes.byref(a))
+    if n < 0:
+        _lib.check(int(n), "altxs_paged_attn")
+    if n:
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        a.ws, a.ws_bytes = ws.data_ptr(), n
+    _launch("altxs_paged_attn", a, dev)
+    return out

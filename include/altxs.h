@@ -594,6 +594,130 @@ int32_t altxs_pack_dense(const float *base, const float *delta, int64_t N, int64
 int32_t altxs_pack_dense32(const float *base, const float *delta, int64_t N, int64_t K, int64_t ld,
                            void *tiled, int64_t tiled_bytes, altxs_stream_t stream);
 
+/* ---- serving from a paged KV cache ------------------------------------------
+ *
+ * The dense cache of altxs_step holds max_len rows per segment whatever the
+ * segment's length.  Here K and V live in pages of page_size tokens (a power of
+ * two from 16 to 1024) that any segment can own:
+ *   key t of segment b is row t % page_size of page table[b * table_width + t / page_size],
+ *   and element d of kv head h of row s of page g is at
+ *   g * *_page + h * *_head + s * *_slot + d   (strides in elements).
+ * A contiguous [n_pages, Hkv, page_size, head_dim] array is the usual layout;
+ * [n_pages, page_size, Hkv, head_dim] is the same with other strides.
+ * New tokens are rows of [T, heads, head_dim] arrays.  With cu = NULL every
+ * segment has T / B of them; else segment b's are rows cu[b] .. cu[b+1]-1
+ * (cu [B+1], ascending, cu[0] = 0; equal entries: an idle segment; rows from
+ * cu[B] on belong to nobody and keep what their outputs held).  Token t of a
+ * segment (counted from 0) has position pos[b] + t, which is its key row.
+ *
+ * The table, pos and cu are read on the device.  What does not fit is never
+ * followed, and flagged in *err (1 = position, 8 = page): a segment whose
+ * positions leave its table (or max_len) or whose cu descends is left out whole
+ * -- nothing appended, zeros as its attention -- and so is a single row whose
+ * position leaves the rope table or whose page id is outside [0, n_pages).  An
+ * attention row that would read such a page takes zeros for its keys and values.
+ */
+
+#define ALTXS_ROPE_INTERLEAVED 1 /* pairs (2i, 2i+1); default (i, i + rot/2) */
+#define ALTXS_ROPE_INVERSE 2     /* the opposite rotation: the gradient of the default one */
+
+/*
+ * Rotary positions of the heads x[T, H, head_dim]: the pairs (a, b) of a
+ * head's first `rot` dims become (a cos + b sin, b cos - a sin) with row pos[t]
+ * of the cos/sin tables [rows, rot/2] -- the step's own sign
+ * (apply_rotary_emb, src/xsa_ttt/model.py:195-206) -- and the other dims are
+ * copied.  Scaling for long contexts is a matter of the tables.  Computed in
+ * fp32, rounded once.  out may be x (equal strides); otherwise they must not
+ * overlap.  A row whose position lies outside the tables is copied unrotated,
+ * and flagged unless it is negative (padding).
+ */
+typedef struct AltxsRopeArgs {
+  const void *x;
+  void *out;
+  const int32_t *pos;      /* [T] */
+  const float *cos, *sin;  /* [rows, rot/2] */
+  int32_t *err;            /* device error word or NULL */
+  int64_t T, rows;
+  int64_t x_tok, x_head, out_tok, out_head; /* strides in elements */
+  int32_t H, head_dim, rot;                 /* rot even, 2 .. head_dim */
+  int32_t dtype;                            /* ALTXS_F32 / ALTXS_BF16 / ALTXS_F16 */
+  int32_t flags;                            /* ALTXS_ROPE_* */
+  int32_t reserved;
+} AltxsRopeArgs;
+int32_t altxs_rope(const AltxsRopeArgs *a, altxs_stream_t stream);
+
+/*
+ * Write new keys and values into their segments' pages; with rot > 0 the keys,
+ * and the queries q (or NULL) into q_out, are rotated by their positions on the
+ * way (as altxs_rope; rope_rows = rows of the tables).  With rot = 0 q must be
+ * NULL.  q_out may be q.  Where two tokens of one call name the same cache row
+ * (segments sharing a page), either one's values are left there.  The paged
+ * form of the KV write of altxs_step; replaces the reference's StaticKV writes
+ * and commit_packed_row (src/xsa_ttt/model.py:259-461, row_commit.py:59-98).
+ */
+typedef struct AltxsPagedAppendArgs {
+  const void *k, *v, *q;
+  void *q_out, *k_cache, *v_cache;
+  const int32_t *table, *pos, *cu;
+  const float *cos, *sin;
+  int32_t *err;
+  int64_t T, n_pages, rope_rows;
+  int64_t k_tok, k_head, v_tok, v_head, q_tok, q_head, q_out_tok, q_out_head;
+  int64_t kc_page, kc_head, kc_slot, vc_page, vc_head, vc_slot;
+  int32_t B, H, Hkv, head_dim, page_size, table_width, rot, dtype, flags;
+  int32_t reserved;
+} AltxsPagedAppendArgs;
+int32_t altxs_paged_append(const AltxsPagedAppendArgs *a, altxs_stream_t stream);
+
+/*
+ * Attention of the new tokens q[T, H, head_dim] (head h reads kv head
+ * h / (H / Hkv)) over their segments' pages, into which their own keys and
+ * values have been appended.  A token at position p of a segment of len =
+ * pos[b] + its new tokens sees the keys [lo, hi):
+ *   hi = max(p + 1, min(prefix[b], len))   prefix: keys seen by every token; NULL = causal
+ *   lo = max(0, p - window + 1, starts[t]) window 0 = off; starts[T]: where the
+ *                                          token's document begins, or NULL
+ * with scores  s = scale * q.k;  s = softcap * tanh(s / softcap) (softcap 0 =
+ * off);  s -= slopes[h] * |p - key| (NULL = off), and out = softmax(s) V; a
+ * token that sees nothing gets zeros.  What lies in rows that a token does not
+ * see (leftovers, infinities, NaN) does not reach it.
+ *
+ * q, the cache and out share dtype.  Scores, the softmax's maximum and sum and
+ * the output are accumulated in fp32; in the 16-bit types the softmax weights
+ * are rounded to the type for the MFMA products.  A row's bits depend on the
+ * row's own query, keys and masks alone -- not on the batch, the chunk it came
+ * in, the pages or the launch -- so encode windows and decode rows agree.
+ *
+ * max_len bounds the keys of a segment (at most table_width * page_size); it
+ * sizes the launch, so pass the real bound when it is known.  ws:
+ * altxs_paged_attn_workspace_bytes(a) bytes, 16-byte aligned, not shared by calls that
+ * may overlap.  Replaces run_split_attn / _static_window_attention
+ * (src/xsa_ttt/split_attn.py:341-425, model.py:550-585) for segments of any
+ * lengths.
+ */
+typedef struct AltxsPagedAttnArgs {
+  const void *q, *k_cache, *v_cache;
+  void *out;
+  const int32_t *table, *pos, *cu;
+  const int32_t *starts;  /* [T] or NULL */
+  const int32_t *prefix;  /* [B] or NULL */
+  const float *slopes;    /* [H] or NULL */
+  int32_t *err;
+  void *ws;
+  int64_t ws_bytes;
+  int64_t T, n_pages;
+  int64_t q_tok, q_head, out_tok, out_head;
+  int64_t kc_page, kc_head, kc_slot, vc_page, vc_head, vc_slot;
+  float scale, softcap;   /* scale > 0; softcap >= 0 */
+  int32_t B, H, Hkv, head_dim, page_size, table_width, max_len, window, dtype;
+  int32_t reserved;
+} AltxsPagedAttnArgs;
+int32_t altxs_paged_attn(const AltxsPagedAttnArgs *a, altxs_stream_t stream);
+
+/* Workspace bytes of altxs_paged_attn for these arguments (host-only; pointers
+ * and strides are not read; <0 on error; 0: ws may be NULL). */
+int64_t altxs_paged_attn_workspace_bytes(const AltxsPagedAttnArgs *a);
+
 #ifdef __cplusplus
 }
 #endif
