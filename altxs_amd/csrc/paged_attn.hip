@@ -3,9 +3,45 @@
 //
 //   y = softmax(s) V,  s_key = bias(scale q . k_key),  key in [lo, hi)
 //
-// One wave per (token, head): 64 keys at a time, a key per lane for the scores
-// and a dim per lane for the sum over V, with the running maximum and sum of the
-// softmax in fp32.
+// The softmax in one pass.  Keys come in tiles of 64 and chunks of 4 tiles.
+// Inside a chunk a running maximum m, sum l and output O are kept over the
+// tiles (m moves only when a tile's maximum passes it by more than 8 powers of
+// two, so O is rarely rescaled; weights stay below 2^8); a chunk starts afresh,
+// and the chunks' (m, l, O) are folded in order:
+//   M' = max(M, m), L' = L 2^(M - M') + l 2^(m - M'), O likewise.
+// Tiles and chunks begin at multiples of their sizes from key 0, so a row's
+// arithmetic is the same wherever its chunks are worked on -- one after the
+// other by a workgroup that keeps the totals, or by workgroups of their own whose
+// partial results a second launch folds.  That makes the bits of a row
+// independent of batch, window width and launch, as in the dense attention, and
+// lets long caches with few rows be split over the whole chip.
+//
+// Products (16-bit types): S^T = K Q^T and O^T = V^T P^T by v_mfma_f32_16x16x32.
+// Lane 16 g + c of a score tile holds, for query row c, keys 16 kb + 4 g + i
+// (kb, i < 4): a row's maximum and sum need two lane exchanges, and the lane's own
+// eight values of blocks 2 s, 2 s + 1 are the P^T operand of step s when the
+// contraction's keys are taken in the order 16 (j / 4) + 4 g + j % 4.  V's operand
+// in that order comes out of row-major V tiles in LDS by ds_read_b64_tr_b16.
+// Rows of a tile are (token, query head of the kv head's group) pairs, token-major:
+// grouped heads and neighbouring tokens share every K and V read.
+//
+// Two kernels, one arithmetic:
+//   few   up to 16 rows a segment and kv head on average (decode): 16-row tiles.  A
+//         workgroup takes a chunk at a time, its four waves a tile each for the
+//         scores (K straight into the operand registers) and a quarter of the
+//         dims each for P V, so a chunk's loads are all in flight at once.
+//   many  128-row tiles, 32 rows a wave; K and V tiles go through LDS, loaded
+//         ahead, and are read by all four waves.
+// fp32 (the framework's exact mode) takes one wave per row, VALU sums.
+//
+// Rows that a tile's rows do not all see.  Scores outside [lo, hi) become -inf.
+// Keys outside the union of the tile's ranges, and keys of bad pages, are loaded
+// from a row of zeros instead.  Only keys between can carry a neighbour's
+// infinities or NaN into a row (0 * inf in P V): tiles with such keys
+// zero V's non-finite elements for the product and add them, times their
+// weights, to the rows that do see them.
+#include <type_traits>
+
 #include "common.h"
 #include "paged.h"
 
@@ -13,12 +49,16 @@ namespace {
 
 using namespace altxs_paged;
 
-constexpr int THREADS = 256, WAVES = THREADS / WAVE, TILE = 64;
+constexpr int THREADS = 256, WAVES = THREADS / WAVE, TILE = 64, CHUNK = 256, TPC = CHUNK / TILE;
+static_assert(TPC == WAVES, "the few-row kernel gives each wave a tile of the chunk");
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LAZY = 8.f;  // how far (powers of two) a tile's maximum passes m before m moves
 
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__bf16 x) { return (float)x; }
 __device__ __forceinline__ float to_f(_Float16 x) { return (float)x; }
+
+alignas(16) static __device__ const uint32_t kZeroRow[64] = {};  // a K or V row of zeros (head_dim <= 128, 16 bits)
 
 struct AttnP {
   const void *q, *k, *v;
@@ -28,9 +68,707 @@ struct AttnP {
   int32_t* err;
   int64_t T, n_pages, q_tok, q_head, o_tok, o_head;
   int64_t kc_page, kc_head, kc_slot, vc_page, vc_head, vc_slot;
-  float scale, softcap;
+  float scale, softcap, scale2;  // scale2 = scale * log2(e)
   int B, W, H, Hkv, G, width, shift, cap, window;
+  FastDiv by_g, by_hkv, by_tiles;  // by_tiles: row tiles of a segment (cu = NULL)
+  // chunk partials: part[(row * nc + c) * HD + d] and ml[row * nc + c], row = t * H + h
+  float* part;
+  float2* ml;
+  int nc;
+  bool direct;  // a workgroup folds all its rows' chunks and writes out
 };
+
+// ---- rows ------------------------------------------------------------------
+
+// A workgroup's row tile: rows r0 .. of segment b (rows of its tokens x group heads).
+struct RowTile {
+  int b, r0, rows;  // rows: of the whole segment; none left when r0 >= rows
+  Segment s;
+};
+
+// Which tile slot `slot` is, of `br` rows; every wave finds it for itself, 64
+// segments per step.  The first workgroup also checks that cu ascends.
+__device__ __forceinline__ RowTile find_tile(const AttnP& a, int slot, int br, int lane, bool first) {
+  RowTile t;
+  int c0, c1;
+  if (a.cu) {
+    int b = 0;
+    bool bad = false;
+    for (int i = 0; i < a.B; i += WAVE) {
+      const int j = i + lane < a.B ? i + lane + 1 : a.B;
+      int c = a.cu[j];
+      if (first) bad = bad || c < a.cu[j - 1] || c > a.T;
+      c = c < 0 ? 0 : c > a.T ? (int)a.T : c;
+      b += __builtin_popcountll(__ballot(i + lane < a.B && first_slot(c, a.G, br, j) <= slot));
+    }
+    if (first && __any(bad) && lane == 0) flag_err(a.err, ALTXS_EDEV_POS);
+    t.b = __builtin_amdgcn_readfirstlane(b);
+    if (t.b >= a.B) {
+      t.r0 = t.rows = 0;
+      return t;
+    }
+    c0 = a.cu[t.b];
+    c1 = a.cu[t.b + 1];
+    t.s = segment_of(c0, c1, a.pos[t.b], a.T, a.cap);
+    const int64_t j = slot - first_slot(t.s.t0, a.G, br, t.b);
+    t.rows = t.s.n * a.G;
+    t.r0 = j < 0 || j * br >= t.rows ? t.rows : (int)(j * br);
+  } else {
+    t.b = (int)div_by(slot, a.by_tiles);
+    c0 = t.b * a.W;
+    t.s = segment_of(c0, c0 + a.W, a.pos[t.b], a.T, a.cap);
+    t.rows = a.W * a.G;
+    t.r0 = (slot - t.b * (int)a.by_tiles.d) * br;
+  }
+  return t;
+}
+
+// One query row as a lane's column sees it.
+struct Row {
+  int lo, hi, p;      // rows past the segment's last: everything is let through, nothing stored
+  float slope2;       // slope * log2(e)
+  int64_t t;          // token
+  int h;              // query head
+  bool valid, empty;  // empty: a valid row that sees nothing
+};
+
+__device__ __forceinline__ Row row_of(const AttnP& a, const RowTile& tile, int hk, int r) {
+  Row o;
+  o.valid = r < tile.rows;
+  const int rr = o.valid ? r : 0;
+  const int i = (int)div_by(rr, a.by_g);
+  o.t = tile.s.t0 + i;
+  o.h = hk * a.G + (rr - i * a.G);
+  o.p = tile.s.pos + i;
+  Range k = {0, 0};
+  if (tile.s.ok)
+    k = keys_seen(o.p, tile.s.pos + tile.s.n, a.window, a.starts ? a.starts[o.t] : 0, a.prefix ? a.prefix[tile.b] : 0);
+  o.empty = o.valid && k.lo >= k.hi;
+  o.lo = o.valid ? k.lo : 0;
+  o.hi = o.valid ? k.hi : INT32_MAX;
+  o.slope2 = a.slopes ? a.slopes[o.h] * LOG2E : 0.f;
+  return o;
+}
+
+__device__ __forceinline__ int row16_imin(int v) {
+#pragma unroll
+  for (int m = 8; m; m >>= 1) {
+    const int o = __shfl_xor(v, m, WAVE);
+    v = v < o ? v : o;
+  }
+  return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int row16_imax(int v) { return -row16_imin(-v); }
+
+// What a set of rows sees: the union [lo, hi) and what all of them see, [clo, chi)
+// (rows that see nothing make it empty).
+struct Seen {
+  int lo, hi, clo, chi;
+  __device__ bool full(int k0) const { return clo <= k0 && chi >= k0 + TILE; }
+  // some key that is loaded (in [LO, HI)) is hidden from some row
+  __device__ bool mixed(int k0, int LO, int HI) const {
+    return clo > (k0 > LO ? k0 : LO) || chi < (k0 + TILE < HI ? k0 + TILE : HI);
+  }
+};
+__device__ __forceinline__ Seen seen_by(const Row& r) {
+  Seen s;
+  const bool some = r.valid && !r.empty;
+  s.lo = row16_imin(some ? r.lo : INT32_MAX);
+  s.hi = row16_imax(some ? r.hi : 0);
+  s.clo = row16_imax(!r.valid ? 0 : r.empty ? INT32_MAX : r.lo);
+  s.chi = row16_imin(!r.valid ? INT32_MAX : r.empty ? 0 : r.hi);
+  return s;
+}
+__device__ __forceinline__ Seen both(const Seen a, const Seen b) {
+  return {a.lo < b.lo ? a.lo : b.lo, a.hi > b.hi ? a.hi : b.hi, a.clo > b.clo ? a.clo : b.clo, a.chi < b.chi ? a.chi : b.chi};
+}
+
+// ---- tile arithmetic ---------------------------------------------------------
+
+template <class T> struct Op;
+template <> struct Op<__bf16> {
+  typedef bf16x8 vec;
+  static constexpr uint32_t EXP = 0x7f807f80u, ONE = 0x00800080u;  // exponent fields of a pair, their lowest bits
+  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
+  }
+};
+template <> struct Op<_Float16> {
+  typedef f16x8 vec;
+  static constexpr uint32_t EXP = 0x7c007c00u, ONE = 0x04000400u;
+  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
+  }
+};
+
+// The weights of a step's 32 keys (score blocks 2 s, 2 s + 1) as its P operand,
+// rounded to the nearest value of the type.
+template <class T>
+__device__ __forceinline__ u32x4 p_operand(const f32x4 a, const f32x4 b) {
+  typename Op<T>::vec v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] = (T)a[i];
+    v[4 + i] = (T)b[i];
+  }
+  return __builtin_bit_cast(u32x4, v);
+}
+
+// Products q.k of a tile -> scores (BIAS: finished, base 2; else still to be scaled by
+// scale2) with -inf outside [lo, hi), and their maximum over the row in the base-2 domain.
+template <bool BIAS>
+__device__ __forceinline__ float tile_scores(const AttnP& a, f32x4 (&S)[4], const Row& r, int k0, int g, bool full) {
+#pragma clang fp contract(off)
+  if constexpr (BIAS) {
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = S[kb][i];
+        if (a.softcap > 0.f) {  // cap tanh(y) log2(e) = cap2 - 2 cap2 / (1 + 2^(2 log2(e) y)), y = scale x / cap
+          const float e = __builtin_amdgcn_exp2f(x * (2.f * a.scale2 / a.softcap));
+          const float cap2 = a.softcap * LOG2E;
+          x = __builtin_fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + e), cap2);
+        } else {
+          x *= a.scale2;
+        }
+        S[kb][i] = __builtin_fmaf(-r.slope2, fabsf((float)(r.p - (k0 + 16 * kb + 4 * g + i))), x);
+      }
+  }
+  if (!full) {
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = k0 + 16 * kb + 4 * g + i;
+        S[kb][i] = key >= r.lo && key < r.hi ? S[kb][i] : -INFINITY;
+      }
+  }
+  float m = S[0][0];
+#pragma unroll
+  for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = fmaxf(m, S[kb][i]);
+  m = rows_max(m);
+  return BIAS ? m : m * a.scale2;
+}
+
+// m after a tile of maximum mx, and the factor of what was summed before.
+__device__ __forceinline__ float next_max(float& m, float mx) {
+#pragma clang fp contract(off)
+  const float old = m;
+  m = mx > old + LAZY ? mx : old;
+  return m == old ? 1.f : __builtin_amdgcn_exp2f(old - m);
+}
+
+// Scores -> weights 2^(s - m); the lane's own sum of them, in a fixed order.
+template <bool BIAS>
+__device__ __forceinline__ float tile_weights(const AttnP& a, f32x4 (&S)[4], float m) {
+#pragma clang fp contract(off)
+  const float mu = m == -INFINITY ? 0.f : m, sc = BIAS ? 1.f : a.scale2;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      S[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[kb][i], sc, -mu));
+      sum[i] += S[kb][i];
+    }
+  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+
+// V tiles in LDS: rows of HD elements whose 16-byte pieces are permuted so that the
+// 32-byte reads of eight consecutive rows fall into different banks.
+template <int HD> __device__ __forceinline__ int v_piece(int row, int piece) {
+  return piece ^ (HD == 64 ? 2 * ((row >> 1) & 3) : 2 * (row & 7));
+}
+// K tiles: a lane reads whole pieces, 16 consecutive rows at the same one.
+template <int HD> __device__ __forceinline__ int k_piece(int row, int piece) {
+  return piece ^ (HD == 64 ? (row >> 1) & 7 : row & 15);
+}
+
+typedef __attribute__((__vector_size__(4 * sizeof(short)))) short i16x4;
+typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+typedef const __attribute__((address_space(1))) void glob_void;
+typedef __attribute__((address_space(3))) void lds_void;
+
+// 16 bytes a lane from global memory straight into LDS (lane l's at dst + 16 l).
+__device__ __forceinline__ void load_lds16(const void* src, void* dst) {
+  __builtin_amdgcn_global_load_lds((glob_void*)src, (lds_void*)dst, 16, 0, 0);
+}
+
+// V operand of step s, dims 16 nb ..: ds_read_b64_tr_b16 gives lane i of each 16
+// lanes element i & 3 of the 8-byte pieces that lanes (i >> 2) + 4 j address, j < 4.
+template <int HD>
+__device__ __forceinline__ u32x4 v_operand(const uint16_t* vt, int s, int nb, int lane) {
+  const int g = lane >> 4, col = lane & 15;
+  u32x2 h[2];
+#pragma unroll
+  for (int jb = 0; jb < 2; ++jb) {
+    const int row = 32 * s + 16 * jb + 4 * g + (col >> 2);
+    const uint16_t* at = vt + row * HD + 8 * v_piece<HD>(row, 2 * nb + ((col & 3) >> 1)) + 4 * (col & 1);
+    h[jb] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)at));
+  }
+  return u32x4{h[0][0], h[0][1], h[1][0], h[1][1]};
+}
+
+// O += P V over one tile, dims 16 (nb0 + nb) ..; O[cb][nb]: row block cb.
+template <class T, int HD, int CB, int NB>
+__device__ __forceinline__ void tile_pv(f32x4 (&O)[CB][NB], const u32x4 (&P)[CB][2], const uint16_t* vt, int nb0, bool mixed,
+                                        const Row (&r)[CB], int k0, int lane) {
+#pragma clang fp contract(off)
+  if (!mixed) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const u32x4 v = v_operand<HD>(vt, s, nb0 + nb, lane);
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) O[cb][nb] = Op<T>::mfma(v, P[cb][s], O[cb][nb]);
+      }
+    return;
+  }
+  uint32_t bad = 0;
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      u32x4 v = v_operand<HD>(vt, s, nb0 + nb, lane);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // a full exponent field carries into the bit above it
+        const uint32_t f = ((v[i] & Op<T>::EXP) + Op<T>::ONE) & 0x80008000u;
+        bad |= f;
+        v[i] &= ~((f >> 15) * 0xffffu);
+      }
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) O[cb][nb] = Op<T>::mfma(v, P[cb][s], O[cb][nb]);
+    }
+  if (__any(bad != 0)) {  // rare: the elements left out, for the rows that see them
+    const int g = lane >> 4, col = lane & 15;
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+      u32x4 w[2] = {P[cb][0], P[cb][1]};
+#pragma unroll 1
+      for (int n = 0; n < 8; ++n) {  // pair n of a lane's weights: keys 16 (n / 2) + 4 g + 2 (n % 2) + {0, 1}
+        const uint32_t pair = w[0][0];
+        w[0] = u32x4{w[0][1], w[0][2], w[0][3], w[1][0]};
+        w[1] = u32x4{w[1][1], w[1][2], w[1][3], pair};
+#pragma unroll 1
+        for (int q = 0; q < 8; ++q) {
+          const int src = q >> 1, half = q & 1;
+          const int row = 16 * (n >> 1) + 4 * src + 2 * (n & 1) + half, key = k0 + row;
+          const uint32_t both = __shfl(pair, 16 * src + col, WAVE);
+          const float p = to_f(__builtin_bit_cast(T, (uint16_t)(half ? both >> 16 : both)));
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            const int d = 16 * (nb0 + nb) + 4 * g;
+            const uint16_t* at = vt + row * HD + 8 * v_piece<HD>(row, d >> 3) + (d & 7);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t x = at[i];
+              const bool odd = (x & Op<T>::EXP & 0xffffu) == (Op<T>::EXP & 0xffffu);
+              if (odd && key >= r[cb].lo && key < r[cb].hi)
+                O[cb][nb][i] = __builtin_fmaf(p, to_f(__builtin_bit_cast(T, (uint16_t)x)), O[cb][nb][i]);
+            }
+          }
+        }
+      }
+    }
+  }
+}
+
+// Fold a chunk's (m, l) into the totals; its O goes by the factors: skip ? O : O fa + o fb.
+struct Fold {
+  float fa, fb;
+  bool skip;
+};
+__device__ __forceinline__ Fold fold(float& M, float& L, float m, float l) {
+#pragma clang fp contract(off)
+  Fold f;
+  f.skip = m == -INFINITY && l == 0.f;  // the row saw nothing of the chunk (or only scores of -inf)
+  const float Mn = fmaxf(M, m);
+  f.fa = M == Mn ? 1.f : __builtin_amdgcn_exp2f(M - Mn);
+  f.fb = m == Mn ? 1.f : __builtin_amdgcn_exp2f(m - Mn);
+  if (!f.skip) {
+    L = __builtin_fmaf(l, f.fb, L * f.fa);
+    M = Mn;
+  }
+  return f;
+}
+__device__ __forceinline__ float folded(const Fold f, float O, float o) {
+#pragma clang fp contract(off)
+  return f.skip ? O : __builtin_fmaf(o, f.fb, O * f.fa);
+}
+
+template <class T>
+__device__ __forceinline__ void store_out(const AttnP& a, const Row& r, int d, const f32x4 o, float inv) {
+#pragma clang fp contract(off)
+  typedef __attribute__((ext_vector_type(4))) T T4;
+  T4 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = (T)(r.empty ? 0.f : o[i] * inv);
+  *(T4*)((T*)a.out + r.t * a.o_tok + r.h * a.o_head + d) = v;
+}
+
+template <int HD>
+__device__ __forceinline__ void store_part(const AttnP& a, const Row& r, int c, int d, const f32x4 o) {
+  *(f32x4*)(a.part + ((r.t * a.H + r.h) * a.nc + c) * HD + d) = o;
+}
+
+// The table entry of a key, read for the nearest key of the rows' union [LO, HI)
+// (LO < HI <= what the table holds), and the page it names: -1 for a key outside the
+// union or an entry that is no page (flagged).
+__device__ __forceinline__ int key_entry(const AttnP& a, int b, int key, int LO, int HI) {
+  const int k = key < LO ? LO : key >= HI ? HI - 1 : key;
+  return a.table[(int64_t)b * a.width + (k >> a.shift)];
+}
+__device__ __forceinline__ int entry_page(const AttnP& a, int entry, int key, int LO, int HI) {
+  const bool seen = key >= LO && key < HI, good = entry >= 0 && entry < a.n_pages;
+  if (seen && !good) flag_err(a.err, ALTXS_EDEV_PAGE);
+  return seen && good ? entry : -1;
+}
+
+// A key's row of kv head hk (head = its offset) in a cache, or the row of zeros.
+template <class T>
+__device__ __forceinline__ const T* key_row(const void* cache, int page, int key, int shift, int64_t st_page, int64_t st_slot,
+                                            int64_t head) {
+  const int64_t at = (int64_t)(page < 0 ? 0 : page) * st_page + head + (int64_t)(key & ((1 << shift) - 1)) * st_slot;
+  const T* p = (const T*)cache + at;
+  return page < 0 ? (const T*)kZeroRow : p;
+}
+
+// ---- few rows ----------------------------------------------------------------
+
+template <class T, int HD, bool BIAS>
+__global__ __launch_bounds__(THREADS) void attn_few_kernel(AttnP a) {
+#pragma clang fp contract(off)
+  constexpr int KS = HD / 32, NB = HD / 16 / WAVES;      // k-steps of a score; 16-dim blocks of a wave's share of O
+  constexpr int PR = HD / 8, RPL = WAVE / PR;            // 16-byte pieces of a row; rows of one LDS load
+  __shared__ alignas(16) uint16_t vt[TPC][TILE * HD];
+  __shared__ u32x4 pt[TPC][2][WAVE];
+  __shared__ float tmax[TPC][16], lsum[TPC][WAVE];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE;
+  const int g = lane >> 4, col = lane & 15;
+  const int slot = (int)div_by(blockIdx.x, a.by_hkv), hk = blockIdx.x - slot * a.Hkv;
+  const RowTile tile = find_tile(a, slot, 16, lane, blockIdx.x == 0 && blockIdx.y == 0 && wave == 0);
+  if (tile.r0 >= tile.rows) return;
+  if (!tile.s.ok && lane == 0) flag_err(a.err, ALTXS_EDEV_POS);
+  const Row row[1] = {row_of(a, tile, hk, tile.r0 + col)};
+  const Row& r = row[0];
+  const Seen seen = seen_by(r);
+  u32x4 q[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+    q[s] = r.valid ? *(const u32x4*)((const T*)a.q + r.t * a.q_tok + r.h * a.q_head + 32 * s + 8 * g) : u32x4{0, 0, 0, 0};
+  float M = -INFINITY, L = 0.f;
+  f32x4 O[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) O[nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int c_end = (seen.hi + CHUNK - 1) / CHUNK;
+  if (seen.lo < seen.hi) {
+    for (int c = seen.lo / CHUNK + blockIdx.y; c < c_end; c += gridDim.y) {
+      const int k0 = c * CHUNK + wave * TILE;
+      const int pg = entry_page(a, key_entry(a, tile.b, k0 + lane, seen.lo, seen.hi), k0 + lane, seen.lo, seen.hi);
+      u32x4 k[4][KS];
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb) {
+        const int i = 16 * kb + col;
+        const T* src = key_row<T>(a.k, __shfl(pg, i, WAVE), k0 + i, a.shift, a.kc_page, a.kc_slot, hk * a.kc_head);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) k[kb][s] = *(const u32x4*)(src + 32 * s + 8 * g);
+      }
+#pragma unroll
+      for (int i = 0; i < TILE / RPL; ++i) {
+        const int vr = i * RPL + lane / PR;
+        const T* src = key_row<T>(a.v, __shfl(pg, vr, WAVE), k0 + vr, a.shift, a.vc_page, a.vc_slot, hk * a.vc_head);
+        load_lds16(src + 8 * v_piece<HD>(vr, lane % PR), vt[wave] + i * RPL * HD);
+      }
+      f32x4 S[4];
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb) {
+        S[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) S[kb] = Op<T>::mfma(k[kb][s], q[s], S[kb]);
+      }
+      const float mx = tile_scores<BIAS>(a, S, r, k0, g, seen.full(k0));
+      if (g == 0) tmax[wave][col] = mx;
+      __syncthreads();
+      float m = -INFINITY, mw = 0.f, al[TPC];
+#pragma unroll
+      for (int t = 0; t < TPC; ++t) {
+        al[t] = next_max(m, tmax[t][col]);
+        if (t == wave) mw = m;
+      }
+      lsum[wave][lane] = tile_weights<BIAS>(a, S, mw);
+      pt[wave][0][lane] = p_operand<T>(S[0], S[1]);
+      pt[wave][1][lane] = p_operand<T>(S[2], S[3]);
+      __builtin_amdgcn_s_waitcnt(0);  // the V tiles
+      __syncthreads();
+      float l = 0.f;
+      f32x4 o[1][NB];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) o[0][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int t = 0; t < TPC; ++t) {
+        l = __builtin_fmaf(l, al[t], lsum[t][lane]);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) o[0][nb] *= al[t];
+        const u32x4 P[1][2] = {{pt[t][0][lane], pt[t][1][lane]}};
+        const int kt = c * CHUNK + t * TILE;
+        tile_pv<T, HD, 1, NB>(o, P, vt[t], wave * NB, seen.mixed(kt, seen.lo, seen.hi), row, kt, lane);
+      }
+      l = rows_sum(l);
+      if (a.direct) {
+        const Fold f = fold(M, L, m, l);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) O[nb][i] = folded(f, O[nb][i], o[0][nb][i]);
+      } else if (r.valid) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) store_part<HD>(a, r, c, 16 * (wave * NB + nb) + 4 * g, o[0][nb]);
+        if (wave == 0 && g == 0) a.ml[(r.t * a.H + r.h) * a.nc + c] = float2{m, l};
+      }
+      __syncthreads();  // the chunk's LDS is free
+    }
+  }
+  if (a.direct && r.valid) {
+    const float inv = 1.f / L;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) store_out<T>(a, r, 16 * (wave * NB + nb) + 4 * g, O[nb], inv);
+  }
+}
+
+// ---- many rows ---------------------------------------------------------------
+
+constexpr int CB = 2, MANY = WAVES * 16 * CB;  // row blocks of a wave; rows of a workgroup
+
+template <class T, int HD, bool BIAS>
+__global__ __launch_bounds__(THREADS, 2) void attn_many_kernel(AttnP a) {
+#pragma clang fp contract(off)
+  constexpr int KS = HD / 32, NB = HD / 16;
+  constexpr int PR = HD / 8, RPL = THREADS / PR, LOADS = TILE / RPL;  // rows of one load of the workgroup; loads of a tile
+  // separate arrays: reads of one buffer do not wait for the loads into the other
+  __shared__ alignas(16) uint16_t kt0[TILE * HD], kt1[TILE * HD], vt0[TILE * HD], vt1[TILE * HD];
+  __shared__ int range[2][WAVES];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE;
+  const int g = lane >> 4, col = lane & 15;
+  const int slot = (int)div_by(blockIdx.x, a.by_hkv), hk = blockIdx.x - slot * a.Hkv;
+  // the last tiles of a segment see the most keys: they go first
+  const RowTile tile = find_tile(a, (int)(gridDim.x / a.Hkv) - 1 - slot, MANY, lane, blockIdx.x == 0 && blockIdx.y == 0 && wave == 0);
+  if (tile.r0 >= tile.rows) return;
+  if (!tile.s.ok && threadIdx.x == 0) flag_err(a.err, ALTXS_EDEV_POS);
+  Row r[CB];
+  u32x4 q[CB][KS];
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb) {
+    r[cb] = row_of(a, tile, hk, tile.r0 + 16 * (wave * CB + cb) + col);
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+      q[cb][s] = r[cb].valid ? *(const u32x4*)((const T*)a.q + r[cb].t * a.q_tok + r[cb].h * a.q_head + 32 * s + 8 * g)
+                             : u32x4{0, 0, 0, 0};
+  }
+  const Seen seen = both(seen_by(r[0]), seen_by(r[1]));
+  if (lane == 0) {
+    range[0][wave] = seen.lo;
+    range[1][wave] = seen.hi;
+  }
+  __syncthreads();
+  int LO = INT32_MAX, HI = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    LO = LO < range[0][w] ? LO : range[0][w];
+    HI = HI > range[1][w] ? HI : range[1][w];
+  }
+  LO = __builtin_amdgcn_readfirstlane(LO);
+  HI = __builtin_amdgcn_readfirstlane(HI);
+
+  float m[CB], l[CB], M[CB], L[CB];
+  f32x4 O[CB][NB], Ot[CB][NB];
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb) {
+    m[cb] = M[cb] = -INFINITY;
+    l[cb] = L[cb] = 0.f;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) O[cb][nb] = Ot[cb][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const int t_end = LO < HI ? (HI + TILE - 1) / TILE : 0, skip = TPC * ((int)gridDim.y - 1);
+  auto after = [&](int t) { return (t + 1) % TPC == 0 ? t + 1 + skip : t + 1; };
+  auto lookup = [&](int t, int (&e)[LOADS]) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) e[i] = key_entry(a, tile.b, t * TILE + i * RPL + threadIdx.x / PR, LO, HI);
+  };
+  auto load = [&](int t, const int (&e)[LOADS], uint16_t* kb, uint16_t* vb) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int row = i * RPL + threadIdx.x / PR, key = t * TILE + row, at = (i * RPL + wave * (RPL / WAVES)) * HD;
+      const int pg = entry_page(a, e[i], key, LO, HI);
+      const T* ks = key_row<T>(a.k, pg, key, a.shift, a.kc_page, a.kc_slot, hk * a.kc_head);
+      const T* vs = key_row<T>(a.v, pg, key, a.shift, a.vc_page, a.vc_slot, hk * a.vc_head);
+      load_lds16(ks + 8 * k_piece<HD>(row, threadIdx.x % PR), kb + at);
+      load_lds16(vs + 8 * v_piece<HD>(row, threadIdx.x % PR), vb + at);
+    }
+  };
+
+  int t = 0;
+  if (LO < HI) {
+    const int c = LO / CHUNK + blockIdx.y;
+    t = blockIdx.y == 0 ? LO / TILE : c * TPC;
+  }
+  // One tile out of (kb, vb), the next one, whose entries are in en, loaded into (kn, vn)
+  // meanwhile, the entries of the one after into ea; false after the last.
+  int tn = 0;
+  auto step = [&](const uint16_t* kb, const uint16_t* vb, uint16_t* kn, uint16_t* vn, const int (&en)[LOADS], int (&ea)[LOADS]) {
+    const int tnn = after(tn);
+    lookup(tnn, ea);
+    if (tn < t_end) load(tn, en, kn, vn);
+    const int k0 = t * TILE;
+    if (seen.lo < k0 + TILE && seen.hi > k0) {  // some row of the wave sees some key of the tile
+      f32x4 S[CB][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) S[cb][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const int row = 16 * j + col;
+          const u32x4 k = *(const u32x4*)(kb + row * HD + 8 * k_piece<HD>(row, 4 * s + g));
+#pragma unroll
+          for (int cb = 0; cb < CB; ++cb) S[cb][j] = Op<T>::mfma(k, q[cb][s], S[cb][j]);
+        }
+      }
+      const bool full = seen.full(k0);
+      u32x4 P[CB][2];
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) {
+        const float al = next_max(m[cb], tile_scores<BIAS>(a, S[cb], r[cb], k0, g, full));
+        l[cb] = __builtin_fmaf(l[cb], al, tile_weights<BIAS>(a, S[cb], m[cb]));
+        P[cb][0] = p_operand<T>(S[cb][0], S[cb][1]);
+        P[cb][1] = p_operand<T>(S[cb][2], S[cb][3]);
+        if (__any(al != 1.f)) {
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) O[cb][nb] *= al;
+        }
+      }
+      tile_pv<T, HD, CB, NB>(O, P, vb, 0, seen.mixed(k0, LO, HI), r, k0, lane);
+    }
+    if (tn >= t_end || tn / TPC != t / TPC) {  // the chunk's last tile
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) {
+        const float ls = rows_sum(l[cb]);
+        if (a.direct) {
+          const Fold f = fold(M[cb], L[cb], m[cb], ls);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) Ot[cb][nb][i] = folded(f, Ot[cb][nb][i], O[cb][nb][i]);
+        } else if (r[cb].valid) {
+          const int c = t / TPC;
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) store_part<HD>(a, r[cb], c, 16 * nb + 4 * g, O[cb][nb]);
+          if (g == 0) a.ml[(r[cb].t * a.H + r[cb].h) * a.nc + c] = float2{m[cb], ls};
+        }
+        m[cb] = -INFINITY;
+        l[cb] = 0.f;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) O[cb][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+    }
+    if (tn >= t_end) return false;
+    __builtin_amdgcn_s_waitcnt(0);  // the next tile is there,
+    __syncthreads();                // and this one's buffer free
+    t = tn;
+    tn = tnn;
+    return true;
+  };
+  if (t < t_end) {
+    int e0[LOADS], e1[LOADS];
+    lookup(t, e0);
+    tn = after(t);
+    lookup(tn, e1);
+    load(t, e0, kt0, vt0);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    while (step(kt0, vt0, kt1, vt1, e1, e0) && step(kt1, vt1, kt0, vt0, e0, e1)) {}
+  }
+  if (a.direct) {
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb)
+      if (r[cb].valid) {
+        const float inv = 1.f / L[cb];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) store_out<T>(a, r[cb], 16 * nb + 4 * g, Ot[cb][nb], inv);
+      }
+  }
+}
+
+// ---- folding the chunks' partial results ---------------------------------------
+
+// The segment of token t (a whole wave asks): -1 behind the last one.
+__device__ __forceinline__ int token_segment(const AttnP& a, int64_t t, int lane, Segment& s) {
+  int b, c0, c1;
+  if (a.cu) {
+    b = 0;
+    for (int i = 0; i < a.B; i += WAVE) b += __builtin_popcountll(__ballot(i + lane < a.B && a.cu[i + lane + 1] <= t));
+    if (b >= a.B) return -1;
+    c0 = a.cu[b];
+    c1 = a.cu[b + 1];
+  } else {
+    b = (int)(t / a.W);
+    c0 = b * a.W;
+    c1 = c0 + a.W;
+  }
+  s = segment_of(c0, c1, a.pos[b], a.T, a.cap);
+  return b;
+}
+
+// One wave per (token, head): its chunks in order, four loads ahead.
+template <class T, int HD>
+__global__ __launch_bounds__(THREADS) void attn_fold_kernel(AttnP a) {
+#pragma clang fp contract(off)
+  constexpr int ND = HD / WAVE;
+  typedef __attribute__((ext_vector_type(ND))) float vec;
+  const int wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE;
+  const int64_t row = (int64_t)blockIdx.x * WAVES + wave;
+  if (row >= a.T * a.H) return;
+  const int64_t t = row / a.H;
+  const int h = (int)(row - t * a.H);
+  Segment s;
+  const int b = token_segment(a, t, lane, s);
+  if (b < 0 || t < s.t0 || t >= s.t0 + s.n) return;
+  Range r = {0, 0};
+  if (s.ok) r = keys_seen(s.pos + (int)(t - s.t0), s.pos + s.n, a.window, a.starts ? a.starts[t] : 0, a.prefix ? a.prefix[b] : 0);
+  float M = -INFINITY, L = 0.f;
+  vec O = 0.f;
+  const float* part = a.part + row * a.nc * HD + lane * ND;
+  const float2* ml = a.ml + row * a.nc;
+  const int c1 = (r.hi + CHUNK - 1) / CHUNK;
+  constexpr int AHEAD = 4;
+  for (int c = r.lo / CHUNK; c < c1; c += AHEAD) {
+    vec o[AHEAD];
+    float2 x[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int cj = c + j < c1 ? c + j : c1 - 1;
+      o[j] = *(const vec*)(part + (int64_t)cj * HD);
+      x[j] = ml[cj];
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (c + j >= c1) break;
+      const Fold f = fold(M, L, x[j].x, x[j].y);
+#pragma unroll
+      for (int i = 0; i < ND; ++i) O[i] = folded(f, O[i], o[j][i]);
+    }
+  }
+  const float inv = 1.f / L;
+  T* out = (T*)a.out + t * a.o_tok + h * a.o_head + lane * ND;
+#pragma unroll
+  for (int i = 0; i < ND; ++i) out[i] = (T)(r.lo < r.hi ? O[i] * inv : 0.f);
+}
+
+// ---- fp32 ----------------------------------------------------------------------
 
 // Scores in the base-2 domain of the softmax: log2(e) (cap tanh(scale x / cap) - slope |p - key|).
 __device__ __forceinline__ float biased(const AttnP& a, float x, float slope, int p, int key) {
@@ -44,6 +782,8 @@ __device__ __forceinline__ float biased(const AttnP& a, float x, float slope, in
   return __builtin_fmaf(-slope * LOG2E, fabsf((float)(p - key)), x);
 }
 
+// One wave per (token, head): a key per lane for the scores, a dim (or two) per lane
+// for the sum over V.
 template <class T, int HD>
 __global__ __launch_bounds__(THREADS) void attn_row_kernel(AttnP a) {
 #pragma clang fp contract(off)
@@ -56,19 +796,9 @@ __global__ __launch_bounds__(THREADS) void attn_row_kernel(AttnP a) {
   if (row >= a.T * a.H) return;
   const int64_t t = row / a.H;
   const int h = (int)(row - t * a.H), hk = h / a.G;
-  int b, c0, c1;
-  if (a.cu) {
-    b = 0;
-    for (int i = 0; i < a.B; i += WAVE) b += __builtin_popcountll(__ballot(i + lane < a.B && a.cu[i + lane + 1] <= t));
-    if (b >= a.B) return;  // behind the last segment
-    c0 = a.cu[b];
-    c1 = a.cu[b + 1];
-  } else {
-    b = (int)(t / a.W);
-    c0 = b * a.W;
-    c1 = c0 + a.W;
-  }
-  const Segment s = segment_of(c0, c1, a.pos[b], a.T, a.cap);
+  Segment s;
+  const int b = token_segment(a, t, lane, s);
+  if (b < 0) return;  // behind the last segment
   Range r = {0, 0};
   const int p = s.pos + (int)(t - s.t0);
   if (s.ok && t >= s.t0)
@@ -118,6 +848,40 @@ __global__ __launch_bounds__(THREADS) void attn_row_kernel(AttnP a) {
   for (int i = 0; i < ND; ++i) out[lane + i * WAVE] = (T)(r.lo < r.hi ? o[i] / l : 0.f);
 }
 
+// ---- host ------------------------------------------------------------------------
+
+// How a call is launched (host decisions only; none of them changes a row's bits).
+struct Plan {
+  bool fp32, few;
+  int nc;       // chunks of max_len
+  int64_t wgs;  // row-tile slots x kv heads
+  int split;    // workgroups that share a row tile's chunks
+  int64_t rows;
+};
+
+Plan plan_of(const AltxsPagedAttnArgs* a) {
+  Plan p = {};
+  p.fp32 = a->dtype == ALTXS_F32;
+  p.rows = a->T * a->H;
+  p.nc = (a->max_len + CHUNK - 1) / CHUNK;
+  if (p.nc < 1) p.nc = 1;
+  p.split = 1;
+  if (p.fp32 || a->T == 0 || a->B == 0) return p;
+  const int G = a->H / a->Hkv;
+  p.few = a->T * G <= 16 * (int64_t)a->B;
+  const int br = p.few ? 16 : MANY;
+  const int64_t slots = a->cu ? slot_count(a->T, G, br, a->B) : (int64_t)a->B * ((a->T / a->B * G + br - 1) / br);
+  p.wgs = slots * a->Hkv;
+  const int64_t fill = p.few ? 2048 : 512, enough = p.few ? 1024 : 384;
+  if (p.wgs < enough) {
+    const int64_t z = (fill + p.wgs - 1) / p.wgs;
+    p.split = (int)(z < p.nc ? z : p.nc);
+  }
+  return p;
+}
+
+int64_t ws_bytes(const Plan& p, int hd) { return p.split > 1 ? ((p.rows * p.nc + 1) / 2 * 4 + p.rows * p.nc * hd) * 4 : 0; }
+
 }  // namespace
 
 static int32_t check(const AltxsPagedAttnArgs* a, const char* who) {
@@ -142,7 +906,7 @@ static int32_t check(const AltxsPagedAttnArgs* a, const char* who) {
 
 extern "C" int64_t altxs_paged_attn_workspace_bytes(const AltxsPagedAttnArgs* a) {
   const int32_t rc = check(a, "altxs_paged_attn_workspace_bytes");
-  return rc ? rc : 0;
+  return rc ? rc : ws_bytes(plan_of(a), a->head_dim);
 }
 
 extern "C" int32_t altxs_paged_attn(const AltxsPagedAttnArgs* a, altxs_stream_t stream) {
@@ -150,6 +914,18 @@ extern "C" int32_t altxs_paged_attn(const AltxsPagedAttnArgs* a, altxs_stream_t 
   if (rc) return rc;
   if (a->T == 0 || a->B == 0) return ALTXS_OK;
   ALTXS_REQUIRE(a->q && a->out && a->k_cache && a->v_cache && a->table && a->pos, "altxs_paged_attn: null pointer");
+  const Plan pl = plan_of(a);
+  if (!pl.fp32) {
+    uintptr_t bits = (uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)a->k_cache | (uintptr_t)a->v_cache;
+    for (int64_t st : {a->q_tok, a->q_head, a->out_tok, a->out_head, a->kc_page, a->kc_head, a->kc_slot, a->vc_page, a->vc_head,
+                       a->vc_slot})
+      bits |= (uintptr_t)(st * 2);
+    ALTXS_REQUIRE((bits & 15) == 0, "altxs_paged_attn: rows of q, out and the caches must start at multiples of 16 bytes");
+  }
+  const int64_t need = ws_bytes(pl, a->head_dim);
+  ALTXS_REQUIRE(need == 0 || (a->ws && a->ws_bytes >= need && ((uintptr_t)a->ws & 15) == 0),
+                "altxs_paged_attn: %lld workspace bytes needed, 16-byte aligned (%lld given)", (long long)need,
+                (long long)a->ws_bytes);
   AttnP p;
   p.q = a->q; p.k = a->k_cache; p.v = a->v_cache; p.out = a->out;
   p.table = a->table; p.pos = a->pos; p.cu = a->cu; p.starts = a->starts; p.prefix = a->prefix;
@@ -157,20 +933,46 @@ extern "C" int32_t altxs_paged_attn(const AltxsPagedAttnArgs* a, altxs_stream_t 
   p.T = a->T; p.n_pages = a->n_pages; p.q_tok = a->q_tok; p.q_head = a->q_head; p.o_tok = a->out_tok; p.o_head = a->out_head;
   p.kc_page = a->kc_page; p.kc_head = a->kc_head; p.kc_slot = a->kc_slot;
   p.vc_page = a->vc_page; p.vc_head = a->vc_head; p.vc_slot = a->vc_slot;
-  p.scale = a->scale; p.softcap = a->softcap;
+  p.scale = a->scale; p.softcap = a->softcap; p.scale2 = a->scale * LOG2E;
   p.B = a->B; p.W = a->cu ? 1 : (int)(a->T / a->B); p.H = a->H; p.Hkv = a->Hkv; p.G = a->H / a->Hkv;
   p.width = a->table_width; p.shift = __builtin_ctz((unsigned)a->page_size); p.cap = a->max_len; p.window = a->window;
-  const dim3 grid((unsigned)((a->T * a->H + WAVES - 1) / WAVES));
+  p.by_g = fast_div(p.G); p.by_hkv = fast_div(p.Hkv);
+  const int br = pl.few ? 16 : MANY;
+  p.by_tiles = fast_div((uint32_t)(((int64_t)p.W * p.G + br - 1) / br));
+  p.nc = pl.nc; p.direct = pl.split == 1;
+  p.ml = (float2*)a->ws;  // then O, from a multiple of 16 bytes on
+  p.part = (float*)a->ws + (pl.rows * pl.nc + 1) / 2 * 4;
   const hipStream_t s = (hipStream_t)stream;
-#define GO(T)                                                                                                   \
-  do {                                                                                                          \
-    if (a->head_dim == 64) hipLaunchKernelGGL((attn_row_kernel<T, 64>), grid, dim3(THREADS), 0, s, p);          \
-    else hipLaunchKernelGGL((attn_row_kernel<T, 128>), grid, dim3(THREADS), 0, s, p);                           \
+  const dim3 block(THREADS), by_row((unsigned)((pl.rows + WAVES - 1) / WAVES));
+  const bool bias = a->softcap > 0.f || a->slopes;
+#define ALTXS_HD_GO(K, ...)                                                          \
+  do {                                                                               \
+    if (a->head_dim == 64) hipLaunchKernelGGL((K<T, 64, ##__VA_ARGS__>), grid, block, 0, s, p);  \
+    else hipLaunchKernelGGL((K<T, 128, ##__VA_ARGS__>), grid, block, 0, s, p);       \
   } while (0)
-  if (a->dtype == ALTXS_F32) GO(float);
-  else if (a->dtype == ALTXS_BF16) GO(__bf16);
-  else GO(_Float16);
-#undef GO
+  if (pl.fp32) {
+    using T = float;
+    const dim3 grid = by_row;
+    ALTXS_HD_GO(attn_row_kernel);
+    ALTXS_CHECK_HIP(hipGetLastError());
+    return ALTXS_OK;
+  }
+  ALTXS_REQUIRE(pl.wgs < (1ll << 31), "altxs_paged_attn: too many row tiles");
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    dim3 grid((unsigned)pl.wgs, (unsigned)pl.split);
+    if (pl.few && bias) ALTXS_HD_GO(attn_few_kernel, true);
+    else if (pl.few) ALTXS_HD_GO(attn_few_kernel, false);
+    else if (bias) ALTXS_HD_GO(attn_many_kernel, true);
+    else ALTXS_HD_GO(attn_many_kernel, false);
+    if (pl.split > 1) {
+      grid = by_row;
+      ALTXS_HD_GO(attn_fold_kernel);
+    }
+  };
+  if (a->dtype == ALTXS_BF16) go(__bf16{});
+  else go(_Float16{});
+#undef ALTXS_HD_GO
   ALTXS_CHECK_HIP(hipGetLastError());
   return ALTXS_OK;
 }
