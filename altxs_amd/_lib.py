@@ -125,7 +125,7 @@ class PagedAppendArgs(ctypes.Structure):
     """AltxsPagedAppendArgs (include/altxs.h)."""
     _fields_ = _fields(p=("k v q q_out k_cache v_cache table pos cu cos sin err", ctypes.c_void_p),
                        i64=("T n_pages rope_rows k_tok k_head v_tok v_head q_tok q_head q_out_tok q_out_head "
-                            "kc_page kc_head kc_slot vc_page vc_head vc_slot", ctypes.c_int64),
+                            "kv_page kv_head kv_slot", ctypes.c_int64),
                        i32=("B H Hkv head_dim page_size table_width rot dtype flags reserved", ctypes.c_int32))
 
 
@@ -133,7 +133,7 @@ class PagedAttnArgs(ctypes.Structure):
     """AltxsPagedAttnArgs (include/altxs.h)."""
     _fields_ = _fields(p=("q k_cache v_cache out table pos cu starts prefix slopes err ws", ctypes.c_void_p),
                        i64=("ws_bytes T n_pages q_tok q_head out_tok out_head "
-                            "kc_page kc_head kc_slot vc_page vc_head vc_slot", ctypes.c_int64),
+                            "kv_page kv_head kv_slot", ctypes.c_int64),
                        f32=("scale softcap", ctypes.c_float),
                        i32=("B H Hkv head_dim page_size table_width max_len window dtype reserved", ctypes.c_int32))
 

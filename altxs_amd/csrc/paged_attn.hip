@@ -67,10 +67,11 @@ struct AttnP {
   const float* slopes;
   int32_t* err;
   int64_t T, n_pages, q_tok, q_head, o_tok, o_head;
-  int64_t kc_page, kc_head, kc_slot, vc_page, vc_head, vc_slot;
+  int64_t kv_head;
+  uint32_t kv_page, kv_slot;
   float scale, softcap, scale2;  // scale2 = scale * log2(e)
   int B, W, H, Hkv, G, width, shift, cap, window;
-  FastDiv by_g, by_hkv, by_tiles;  // by_tiles: row tiles of a segment (cu = NULL)
+  FastDiv by_g, by_hkv, by_b, by_tiles;  // by_tiles: row tiles of a segment (cu = NULL)
   // chunk partials: part[(row * nc + c) * HD + d] and ml[row * nc + c], row = t * H + h
   float* part;
   float2* ml;
@@ -151,11 +152,11 @@ __device__ __forceinline__ Row row_of(const AttnP& a, const RowTile& tile, int h
 }
 
 __device__ __forceinline__ int row16_imin(int v) {
-#pragma unroll
-  for (int m = 8; m; m >>= 1) {
-    const int o = __shfl_xor(v, m, WAVE);
-    v = v < o ? v : o;
-  }
+  auto least = [](int a, int b) { return a < b ? a : b; };
+  v = least(v, (int)dpp_u<DPP_XOR1>((uint32_t)v));
+  v = least(v, (int)dpp_u<DPP_XOR2>((uint32_t)v));
+  v = least(v, (int)dpp_u<DPP_HALF_MIRROR>((uint32_t)v));
+  v = least(v, (int)dpp_u<DPP_MIRROR>((uint32_t)v));
   return __builtin_amdgcn_readfirstlane(v);
 }
 __device__ __forceinline__ int row16_imax(int v) { return -row16_imin(-v); }
@@ -185,17 +186,25 @@ __device__ __forceinline__ Seen both(const Seen a, const Seen b) {
 
 // ---- tile arithmetic ---------------------------------------------------------
 
+// The same value, where rare paths start from it: what they compute stays in them
+// instead of being kept in registers over the whole loop.
+__device__ __forceinline__ int unhoisted(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 template <class T> struct Op;
 template <> struct Op<__bf16> {
   typedef bf16x8 vec;
   static constexpr uint32_t EXP = 0x7f807f80u, ONE = 0x00800080u;  // exponent fields of a pair, their lowest bits
+  static constexpr uint32_t ONES = 0x3f803f80u;                    // a pair of ones
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
   }
 };
 template <> struct Op<_Float16> {
   typedef f16x8 vec;
-  static constexpr uint32_t EXP = 0x7c007c00u, ONE = 0x04000400u;
+  static constexpr uint32_t EXP = 0x7c007c00u, ONE = 0x04000400u, ONES = 0x3c003c00u;
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
   }
@@ -214,43 +223,64 @@ __device__ __forceinline__ u32x4 p_operand(const f32x4 a, const f32x4 b) {
   return __builtin_bit_cast(u32x4, v);
 }
 
+// The larger of two, NaN left out (fmaxf on values out of lane swaps would quiet them first).
+__device__ __forceinline__ float max2(uint32_t a, uint32_t b) {
+  return __builtin_amdgcn_fmed3f(__uint_as_float(a), __uint_as_float(b), INFINITY);
+}
+
 // Products q.k of a tile -> scores (BIAS: finished, base 2; else still to be scaled by
-// scale2) with -inf outside [lo, hi), and their maximum over the row in the base-2 domain.
-template <bool BIAS>
-__device__ __forceinline__ float tile_scores(const AttnP& a, f32x4 (&S)[4], const Row& r, int k0, int g, bool full) {
+// scale2) with -inf outside [lo, hi), and mx, their maximum over the row in the base-2 domain.
+template <bool BIAS, int CB>
+__device__ __forceinline__ void tile_scores(const AttnP& a, f32x4 (&S)[CB][4], float (&mx)[CB], const Row (&r)[CB], int k0, int g,
+                                            bool full) {
 #pragma clang fp contract(off)
   if constexpr (BIAS) {
+    if (a.softcap > 0.f) {  // cap tanh(y) log2(e) = cap2 - 2 cap2 / (1 + 2^(2 log2(e) y)), y = scale x / cap
+      const float e2 = 2.f * a.scale2 / a.softcap, cap2 = a.softcap * LOG2E;
 #pragma unroll
-    for (int kb = 0; kb < 4; ++kb)
+      for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x = S[kb][i];
-        if (a.softcap > 0.f) {  // cap tanh(y) log2(e) = cap2 - 2 cap2 / (1 + 2^(2 log2(e) y)), y = scale x / cap
-          const float e = __builtin_amdgcn_exp2f(x * (2.f * a.scale2 / a.softcap));
-          const float cap2 = a.softcap * LOG2E;
-          x = __builtin_fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + e), cap2);
-        } else {
-          x *= a.scale2;
+        for (int n = 0; n < 16; ++n) {
+          const float e = __builtin_amdgcn_exp2f(S[cb][n / 4][n % 4] * e2);
+          S[cb][n / 4][n % 4] = __builtin_fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + e), cap2);
         }
-        S[kb][i] = __builtin_fmaf(-r.slope2, fabsf((float)(r.p - (k0 + 16 * kb + 4 * g + i))), x);
+    } else {
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+        for (int n = 0; n < 16; ++n) S[cb][n / 4][n % 4] *= a.scale2;
+    }
+    if (a.slopes) {
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) {
+        const int d0 = r[cb].p - (k0 + 4 * g);
+#pragma unroll
+        for (int n = 0; n < 16; ++n)
+          S[cb][n / 4][n % 4] = __builtin_fmaf(-r[cb].slope2, fabsf((float)(d0 - (16 * (n / 4) + n % 4))), S[cb][n / 4][n % 4]);
       }
+    }
   }
   if (!full) {
 #pragma unroll
-    for (int kb = 0; kb < 4; ++kb)
+    for (int cb = 0; cb < CB; ++cb) {
+      // keys lo .. hi - 1 of the lane's own: one comparison each, unsigned
+      const uint32_t lo = r[cb].lo - (k0 + 4 * g), n_seen = r[cb].hi - r[cb].lo;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = k0 + 16 * kb + 4 * g + i;
-        S[kb][i] = key >= r.lo && key < r.hi ? S[kb][i] : -INFINITY;
-      }
+      for (int n = 0; n < 16; ++n)
+        S[cb][n / 4][n % 4] = (uint32_t)(16 * (n / 4) + n % 4) - lo < n_seen ? S[cb][n / 4][n % 4] : -INFINITY;
+    }
   }
-  float m = S[0][0];
 #pragma unroll
-  for (int kb = 0; kb < 4; ++kb)
+  for (int cb = 0; cb < CB; ++cb) {
+    float m = S[cb][0][0];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m = fmaxf(m, S[kb][i]);
-  m = rows_max(m);
-  return BIAS ? m : m * a.scale2;
+    for (int n = 1; n < 16; ++n) m = fmaxf(m, S[cb][n / 4][n % 4]);
+    const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+    m = max2(x[0], x[1]);
+    const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+    m = max2(y[0], y[1]);
+    mx[cb] = BIAS ? m : m * a.scale2;
+  }
 }
 
 // m after a tile of maximum mx, and the factor of what was summed before.
@@ -261,20 +291,18 @@ __device__ __forceinline__ float next_max(float& m, float mx) {
   return m == old ? 1.f : __builtin_amdgcn_exp2f(old - m);
 }
 
-// Scores -> weights 2^(s - m); the lane's own sum of them, in a fixed order.
-template <bool BIAS>
-__device__ __forceinline__ float tile_weights(const AttnP& a, f32x4 (&S)[4], float m) {
+// Scores -> weights 2^(s - m), as the P operands of the tile's two steps.
+template <class T, bool BIAS>
+__device__ __forceinline__ void tile_weights(const AttnP& a, const f32x4 (&S)[4], float m, u32x4 (&P)[2]) {
 #pragma clang fp contract(off)
   const float mu = m == -INFINITY ? 0.f : m, sc = BIAS ? 1.f : a.scale2;
-  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  f32x4 w[4];
 #pragma unroll
   for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      S[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[kb][i], sc, -mu));
-      sum[i] += S[kb][i];
-    }
-  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    for (int i = 0; i < 4; ++i) w[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[kb][i], sc, -mu));
+  P[0] = p_operand<T>(w[0], w[1]);
+  P[1] = p_operand<T>(w[2], w[3]);
 }
 
 // V tiles in LDS: rows of HD elements whose 16-byte pieces are permuted so that the
@@ -291,6 +319,7 @@ typedef __attribute__((__vector_size__(4 * sizeof(short)))) short i16x4;
 typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
 typedef const __attribute__((address_space(1))) void glob_void;
 typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(4))) int32_t const_i32;  // read by scalar loads
 
 // 16 bytes a lane from global memory straight into LDS (lane l's at dst + 16 l).
 __device__ __forceinline__ void load_lds16(const void* src, void* dst) {
@@ -312,11 +341,27 @@ __device__ __forceinline__ u32x4 v_operand(const uint16_t* vt, int s, int nb, in
   return u32x4{h[0][0], h[0][1], h[1][0], h[1][1]};
 }
 
-// O += P V over one tile, dims 16 (nb0 + nb) ..; O[cb][nb]: row block cb.
+// O += P V over one tile, dims 16 (nb0 + nb) ..; O[cb][nb]: row block cb.  l += the
+// sum of the weights, a product with ones: every register holds the row's sum (of the
+// rounded weights, so that they add up to one after the division).
 template <class T, int HD, int CB, int NB>
-__device__ __forceinline__ void tile_pv(f32x4 (&O)[CB][NB], const u32x4 (&P)[CB][2], const uint16_t* vt, int nb0, bool mixed,
-                                        const Row (&r)[CB], int k0, int lane) {
+__device__ __forceinline__ void tile_pv(f32x4 (&O)[CB][NB], f32x4 (&l)[CB], const u32x4 (&P)[CB][2], const uint16_t* vt, int nb0,
+                                        bool mixed, const Row (&r)[CB], int k0, int lane) {
 #pragma clang fp contract(off)
+  constexpr uint32_t ONES = Op<T>::ONES;
+  const u32x4 ones = {ONES, ONES, ONES, ONES};
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) l[cb] = Op<T>::mfma(ones, P[cb][s], l[cb]);
+  if (mixed) {  // does V hold infinities or NaN?  Their sums with anything do (and large sums may: no harm)
+    f32x4 z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) z = Op<T>::mfma(v_operand<HD>(vt, s, nb0 + nb, lane), ones, z);
+    mixed = __any(!(fabsf(z[0]) < INFINITY && fabsf(z[1]) < INFINITY && fabsf(z[2]) < INFINITY && fabsf(z[3]) < INFINITY));
+  }
   if (!mixed) {
 #pragma unroll
     for (int s = 0; s < 2; ++s)
@@ -326,24 +371,21 @@ __device__ __forceinline__ void tile_pv(f32x4 (&O)[CB][NB], const u32x4 (&P)[CB]
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) O[cb][nb] = Op<T>::mfma(v, P[cb][s], O[cb][nb]);
       }
-    return;
-  }
-  uint32_t bad = 0;
+  } else {  // rare: without those elements, which then go to the rows that see them
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      u32x4 v = v_operand<HD>(vt, s, nb0 + nb, lane);
+      for (int nb = 0; nb < NB; ++nb) {
+        u32x4 v = v_operand<HD>(vt, s, nb0 + nb, lane);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {  // a full exponent field carries into the bit above it
-        const uint32_t f = ((v[i] & Op<T>::EXP) + Op<T>::ONE) & 0x80008000u;
-        bad |= f;
-        v[i] &= ~((f >> 15) * 0xffffu);
+        for (int i = 0; i < 4; ++i) {  // a full exponent field carries into the bit above it
+          const uint32_t f = ((v[i] & Op<T>::EXP) + Op<T>::ONE) & 0x80008000u;
+          v[i] &= ~((f << 1) - (f >> 15));
+        }
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) O[cb][nb] = Op<T>::mfma(v, P[cb][s], O[cb][nb]);
       }
-#pragma unroll
-      for (int cb = 0; cb < CB; ++cb) O[cb][nb] = Op<T>::mfma(v, P[cb][s], O[cb][nb]);
-    }
-  if (__any(bad != 0)) {  // rare: the elements left out, for the rows that see them
+    lane = unhoisted(lane);
     const int g = lane >> 4, col = lane & 15;
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {
@@ -377,27 +419,23 @@ __device__ __forceinline__ void tile_pv(f32x4 (&O)[CB][NB], const u32x4 (&P)[CB]
   }
 }
 
-// Fold a chunk's (m, l) into the totals; its O goes by the factors: skip ? O : O fa + o fb.
+// Fold a chunk's (m, l) into the totals; its O goes by the factors: O fa + o fb.
 struct Fold {
   float fa, fb;
-  bool skip;
 };
 __device__ __forceinline__ Fold fold(float& M, float& L, float m, float l) {
 #pragma clang fp contract(off)
   Fold f;
-  f.skip = m == -INFINITY && l == 0.f;  // the row saw nothing of the chunk (or only scores of -inf)
   const float Mn = fmaxf(M, m);
   f.fa = M == Mn ? 1.f : __builtin_amdgcn_exp2f(M - Mn);
-  f.fb = m == Mn ? 1.f : __builtin_amdgcn_exp2f(m - Mn);
-  if (!f.skip) {
-    L = __builtin_fmaf(l, f.fb, L * f.fa);
-    M = Mn;
-  }
+  f.fb = m == Mn ? 1.f : __builtin_amdgcn_exp2f(m - Mn);  // 0 where the row saw nothing of the chunk
+  L = __builtin_fmaf(l, f.fb, L * f.fa);
+  M = Mn;
   return f;
 }
 __device__ __forceinline__ float folded(const Fold f, float O, float o) {
 #pragma clang fp contract(off)
-  return f.skip ? O : __builtin_fmaf(o, f.fb, O * f.fa);
+  return __builtin_fmaf(o, f.fb, O * f.fa);
 }
 
 template <class T>
@@ -430,9 +468,9 @@ __device__ __forceinline__ int entry_page(const AttnP& a, int entry, int key, in
 
 // A key's row of kv head hk (head = its offset) in a cache, or the row of zeros.
 template <class T>
-__device__ __forceinline__ const T* key_row(const void* cache, int page, int key, int shift, int64_t st_page, int64_t st_slot,
+__device__ __forceinline__ const T* key_row(const void* cache, int page, int key, int shift, uint32_t st_page, uint32_t st_slot,
                                             int64_t head) {
-  const int64_t at = (int64_t)(page < 0 ? 0 : page) * st_page + head + (int64_t)(key & ((1 << shift) - 1)) * st_slot;
+  const int64_t at = (int64_t)((uint64_t)(page < 0 ? 0 : page) * st_page + (uint64_t)(key & ((1 << shift) - 1)) * st_slot) + head;
   const T* p = (const T*)cache + at;
   return page < 0 ? (const T*)kZeroRow : p;
 }
@@ -446,7 +484,7 @@ __global__ __launch_bounds__(THREADS) void attn_few_kernel(AttnP a) {
   constexpr int PR = HD / 8, RPL = WAVE / PR;            // 16-byte pieces of a row; rows of one LDS load
   __shared__ alignas(16) uint16_t vt[TPC][TILE * HD];
   __shared__ u32x4 pt[TPC][2][WAVE];
-  __shared__ float tmax[TPC][16], lsum[TPC][WAVE];
+  __shared__ float tmax[TPC][16];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE;
   const int g = lane >> 4, col = lane & 15;
   const int slot = (int)div_by(blockIdx.x, a.by_hkv), hk = blockIdx.x - slot * a.Hkv;
@@ -473,25 +511,26 @@ __global__ __launch_bounds__(THREADS) void attn_few_kernel(AttnP a) {
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb) {
         const int i = 16 * kb + col;
-        const T* src = key_row<T>(a.k, __shfl(pg, i, WAVE), k0 + i, a.shift, a.kc_page, a.kc_slot, hk * a.kc_head);
+        const T* src = key_row<T>(a.k, __shfl(pg, i, WAVE), k0 + i, a.shift, a.kv_page, a.kv_slot, hk * a.kv_head);
 #pragma unroll
         for (int s = 0; s < KS; ++s) k[kb][s] = *(const u32x4*)(src + 32 * s + 8 * g);
       }
 #pragma unroll
       for (int i = 0; i < TILE / RPL; ++i) {
         const int vr = i * RPL + lane / PR;
-        const T* src = key_row<T>(a.v, __shfl(pg, vr, WAVE), k0 + vr, a.shift, a.vc_page, a.vc_slot, hk * a.vc_head);
+        const T* src = key_row<T>(a.v, __shfl(pg, vr, WAVE), k0 + vr, a.shift, a.kv_page, a.kv_slot, hk * a.kv_head);
         load_lds16(src + 8 * v_piece<HD>(vr, lane % PR), vt[wave] + i * RPL * HD);
       }
-      f32x4 S[4];
+      f32x4 S[1][4];
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb) {
-        S[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+        S[0][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < KS; ++s) S[kb] = Op<T>::mfma(k[kb][s], q[s], S[kb]);
+        for (int s = 0; s < KS; ++s) S[0][kb] = Op<T>::mfma(k[kb][s], q[s], S[0][kb]);
       }
-      const float mx = tile_scores<BIAS>(a, S, r, k0, g, seen.full(k0));
-      if (g == 0) tmax[wave][col] = mx;
+      float mx[1];
+      tile_scores<BIAS, 1>(a, S, mx, row, k0, g, seen.full(k0));
+      if (g == 0) tmax[wave][col] = mx[0];
       __syncthreads();
       float m = -INFINITY, mw = 0.f, al[TPC];
 #pragma unroll
@@ -499,27 +538,26 @@ __global__ __launch_bounds__(THREADS) void attn_few_kernel(AttnP a) {
         al[t] = next_max(m, tmax[t][col]);
         if (t == wave) mw = m;
       }
-      lsum[wave][lane] = tile_weights<BIAS>(a, S, mw);
-      pt[wave][0][lane] = p_operand<T>(S[0], S[1]);
-      pt[wave][1][lane] = p_operand<T>(S[2], S[3]);
+      u32x4 w[2];
+      tile_weights<T, BIAS>(a, S[0], mw, w);
+      pt[wave][0][lane] = w[0];
+      pt[wave][1][lane] = w[1];
       __builtin_amdgcn_s_waitcnt(0);  // the V tiles
       __syncthreads();
-      float l = 0.f;
-      f32x4 o[1][NB];
+      f32x4 l[1] = {f32x4{0.f, 0.f, 0.f, 0.f}}, o[1][NB];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) o[0][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int t = 0; t < TPC; ++t) {
-        l = __builtin_fmaf(l, al[t], lsum[t][lane]);
+        l[0] *= al[t];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) o[0][nb] *= al[t];
         const u32x4 P[1][2] = {{pt[t][0][lane], pt[t][1][lane]}};
         const int kt = c * CHUNK + t * TILE;
-        tile_pv<T, HD, 1, NB>(o, P, vt[t], wave * NB, seen.mixed(kt, seen.lo, seen.hi), row, kt, lane);
+        tile_pv<T, HD, 1, NB>(o, l, P, vt[t], wave * NB, seen.mixed(kt, seen.lo, seen.hi), row, kt, lane);
       }
-      l = rows_sum(l);
       if (a.direct) {
-        const Fold f = fold(M, L, m, l);
+        const Fold f = fold(M, L, m, l[0][0]);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -527,7 +565,7 @@ __global__ __launch_bounds__(THREADS) void attn_few_kernel(AttnP a) {
       } else if (r.valid) {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) store_part<HD>(a, r, c, 16 * (wave * NB + nb) + 4 * g, o[0][nb]);
-        if (wave == 0 && g == 0) a.ml[(r.t * a.H + r.h) * a.nc + c] = float2{m, l};
+        if (wave == 0 && g == 0) a.ml[(r.t * a.H + r.h) * a.nc + c] = float2{m, l[0][0]};
       }
       __syncthreads();  // the chunk's LDS is free
     }
@@ -541,21 +579,32 @@ __global__ __launch_bounds__(THREADS) void attn_few_kernel(AttnP a) {
 
 // ---- many rows ---------------------------------------------------------------
 
-constexpr int CB = 2, MANY = WAVES * 16 * CB;  // row blocks of a wave; rows of a workgroup
+constexpr int NW = 4;  // waves of a workgroup
+// 16-row blocks of a wave, and rows of a workgroup
+template <int HD> constexpr int many_cb = HD == 64 ? 2 : 1;
+template <int HD> constexpr int many_rows = NW * 16 * many_cb<HD>;
+
+// The last row tiles of a segment see the most keys: they go first -- of equal segments
+// all last tiles, then all second to last ones; of ragged ones the slots backwards.
+__device__ __forceinline__ int many_slot(const AttnP& a, int i) {
+  if (a.cu) return (int)(gridDim.x / a.Hkv) - 1 - i;
+  const int back = (int)div_by(i, a.by_b), b = i - back * a.B;
+  return (b + 1) * (int)a.by_tiles.d - 1 - back;
+}
 
 template <class T, int HD, bool BIAS>
-__global__ __launch_bounds__(THREADS, 2) void attn_many_kernel(AttnP a) {
+__global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
 #pragma clang fp contract(off)
-  constexpr int KS = HD / 32, NB = HD / 16;
-  constexpr int PR = HD / 8, RPL = THREADS / PR, LOADS = TILE / RPL;  // rows of one load of the workgroup; loads of a tile
+  constexpr int CB = many_cb<HD>, MANY = many_rows<HD>, KS = HD / 32, NB = HD / 16;
+  constexpr int PR = HD / 8, RPW = WAVE / PR, RPL = NW * RPW, LOADS = TILE / RPL;  // rows of a wave's load, of the workgroup's; loads
+  static_assert(RPL % 16 == 0 && RPW <= 16, "a load's rows lie in one page, its pieces are permuted alike");
   // separate arrays: reads of one buffer do not wait for the loads into the other
   __shared__ alignas(16) uint16_t kt0[TILE * HD], kt1[TILE * HD], vt0[TILE * HD], vt1[TILE * HD];
-  __shared__ int range[2][WAVES];
+  __shared__ int range[4][NW];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE;
   const int g = lane >> 4, col = lane & 15;
   const int slot = (int)div_by(blockIdx.x, a.by_hkv), hk = blockIdx.x - slot * a.Hkv;
-  // the last tiles of a segment see the most keys: they go first
-  const RowTile tile = find_tile(a, (int)(gridDim.x / a.Hkv) - 1 - slot, MANY, lane, blockIdx.x == 0 && blockIdx.y == 0 && wave == 0);
+  const RowTile tile = find_tile(a, many_slot(a, slot), MANY, lane, blockIdx.x == 0 && blockIdx.y == 0 && wave == 0);
   if (tile.r0 >= tile.rows) return;
   if (!tile.s.ok && threadIdx.x == 0) flag_err(a.err, ALTXS_EDEV_POS);
   Row r[CB];
@@ -568,113 +617,171 @@ __global__ __launch_bounds__(THREADS, 2) void attn_many_kernel(AttnP a) {
       q[cb][s] = r[cb].valid ? *(const u32x4*)((const T*)a.q + r[cb].t * a.q_tok + r[cb].h * a.q_head + 32 * s + 8 * g)
                              : u32x4{0, 0, 0, 0};
   }
-  const Seen seen = both(seen_by(r[0]), seen_by(r[1]));
+  Seen seen = seen_by(r[0]);
+#pragma unroll
+  for (int cb = 1; cb < CB; ++cb) seen = both(seen, seen_by(r[cb]));
   if (lane == 0) {
     range[0][wave] = seen.lo;
     range[1][wave] = seen.hi;
+    range[2][wave] = seen.clo;
+    range[3][wave] = seen.chi;
   }
   __syncthreads();
-  int LO = INT32_MAX, HI = 0;
+  Seen all = {INT32_MAX, 0, 0, INT32_MAX};
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    LO = LO < range[0][w] ? LO : range[0][w];
-    HI = HI > range[1][w] ? HI : range[1][w];
-  }
-  LO = __builtin_amdgcn_readfirstlane(LO);
-  HI = __builtin_amdgcn_readfirstlane(HI);
+  for (int w = 0; w < NW; ++w) all = both(all, Seen{range[0][w], range[1][w], range[2][w], range[3][w]});
+  const int LO = __builtin_amdgcn_readfirstlane(all.lo), HI = __builtin_amdgcn_readfirstlane(all.hi);
+  // tiles [in0, in1) are seen whole by every row of the workgroup
+  const int in0 = (__builtin_amdgcn_readfirstlane(all.clo < INT32_MAX - TILE ? all.clo : INT32_MAX - TILE) + TILE - 1) / TILE;
+  const int in1 = __builtin_amdgcn_readfirstlane(all.chi) / TILE;
 
-  float m[CB], l[CB], M[CB], L[CB];
-  f32x4 O[CB][NB], Ot[CB][NB];
+  float m[CB], M[CB], L[CB];
+  f32x4 l[CB], O[CB][NB], Ot[CB][NB];
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb) {
     m[cb] = M[cb] = -INFINITY;
-    l[cb] = L[cb] = 0.f;
+    L[cb] = 0.f;
+    l[cb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) O[cb][nb] = Ot[cb][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
   const int t_end = LO < HI ? (HI + TILE - 1) / TILE : 0, skip = TPC * ((int)gridDim.y - 1);
-  auto after = [&](int t) { return (t + 1) % TPC == 0 ? t + 1 + skip : t + 1; };
+  auto after = [&](int t) { return (t & (TPC - 1)) == TPC - 1 ? t + 1 + skip : t + 1; };
+  // Loads go by whole waves, 8 (4) rows at a time, all in one page, whose entry is a
+  // scalar; with pages of a tile or more one entry serves the whole tile.  Entries are
+  // read for the nearest tile or key of the union (inside the table).
+  const const_i32* entries = (const const_i32*)(a.table + (int64_t)tile.b * a.width);
+  const bool large = a.shift >= 6;
   auto lookup = [&](int t, int (&e)[LOADS]) {
+    if (large) {
+      const int entry = entries[(t < t_end ? t : t_end - 1) >> (a.shift - 6)];
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) e[i] = key_entry(a, tile.b, t * TILE + i * RPL + threadIdx.x / PR, LO, HI);
+      for (int i = 0; i < LOADS; ++i) e[i] = entry;
+    } else {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        int key = t * TILE + i * RPL + wave * RPW;
+        key = key < LO ? LO : key >= HI ? HI - 1 : key;
+        e[i] = entries[key >> a.shift];
+      }
+    }
   };
+  const uint32_t n_pages = a.n_pages < INT32_MAX ? (uint32_t)a.n_pages : INT32_MAX;
+  const int whole0 = (LO + TILE - 1) / TILE;  // tiles all of whose keys are in the union
+  const uint32_t wholes = HI / TILE > whole0 ? HI / TILE - whole0 : 0;
+  const int krow = wave * RPW + lane / PR;
+  const T* kl = (const T*)a.k + hk * a.kv_head + (uint64_t)krow * a.kv_slot + 8 * k_piece<HD>(krow, lane % PR);
+  const T* vl = (const T*)a.v + hk * a.kv_head + (uint64_t)krow * a.kv_slot + 8 * v_piece<HD>(krow, lane % PR);
+  const uint64_t down = RPL * (uint64_t)a.kv_slot;  // a load's rows to the next one's
   auto load = [&](int t, const int (&e)[LOADS], uint16_t* kb, uint16_t* vb) {
+    const bool whole = (uint32_t)(t - whole0) < wholes;
+    if (large && whole && (uint32_t)e[0] < n_pages) {
+      uint64_t at = (uint64_t)(uint32_t)e[0] * a.kv_page + (uint64_t)(uint32_t)((t << 6) & ((1 << a.shift) - 1)) * a.kv_slot;
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i, at += down) {
+        const int to = (i * RPL + wave * RPW) * HD;
+        load_lds16(kl + at, kb + to);
+        load_lds16(vl + at, vb + to);
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int row = i * RPL + threadIdx.x / PR, key = t * TILE + row, at = (i * RPL + wave * (RPL / WAVES)) * HD;
-      const int pg = entry_page(a, e[i], key, LO, HI);
-      const T* ks = key_row<T>(a.k, pg, key, a.shift, a.kc_page, a.kc_slot, hk * a.kc_head);
-      const T* vs = key_row<T>(a.v, pg, key, a.shift, a.vc_page, a.vc_slot, hk * a.vc_head);
-      load_lds16(ks + 8 * k_piece<HD>(row, threadIdx.x % PR), kb + at);
-      load_lds16(vs + 8 * v_piece<HD>(row, threadIdx.x % PR), vb + at);
+      const int first = i * RPL, key = t * TILE + first + wave * RPW, entry = e[i];
+      const bool good = (uint32_t)entry < n_pages;
+      // kl and vl already stand krow rows into the page
+      const uint64_t at = (uint64_t)(good ? (uint32_t)entry : 0) * a.kv_page +
+                          (int64_t)((key & ((1 << a.shift) - 1)) - wave * RPW) * (int64_t)a.kv_slot;
+      const T* ks = kl + at;
+      const T* vs = vl + at;
+      const int to = (first + wave * RPW) * HD;
+      if (!(whole && good)) {
+        const int ln = unhoisted(lane), row = wave * RPW + ln / PR;
+        const bool in = key + ln / PR >= LO && key + ln / PR < HI;
+        if (in && !good) flag_err(a.err, ALTXS_EDEV_PAGE);
+        if (!in || !good) {
+          ks = (const T*)kZeroRow + 8 * k_piece<HD>(row, ln % PR);
+          vs = (const T*)kZeroRow + 8 * v_piece<HD>(row, ln % PR);
+        }
+      }
+      load_lds16(ks, kb + to);
+      load_lds16(vs, vb + to);
     }
   };
 
-  int t = 0;
-  if (LO < HI) {
-    const int c = LO / CHUNK + blockIdx.y;
-    t = blockIdx.y == 0 ? LO / TILE : c * TPC;
-  }
-  // One tile out of (kb, vb), the next one, whose entries are in en, loaded into (kn, vn)
-  // meanwhile, the entries of the one after into ea; false after the last.
-  int tn = 0;
-  auto step = [&](const uint16_t* kb, const uint16_t* vb, uint16_t* kn, uint16_t* vn, const int (&en)[LOADS], int (&ea)[LOADS]) {
-    const int tnn = after(tn);
-    lookup(tnn, ea);
-    if (tn < t_end) load(tn, en, kn, vn);
+  int t = 0, tn = 0;
+  // One tile out of (kb, vb).  EDGE: some row does not see it whole.
+  auto work = [&](auto edge, const uint16_t* kb, const uint16_t* vb) {
+    constexpr bool EDGE = decltype(edge)::value;
     const int k0 = t * TILE;
-    if (seen.lo < k0 + TILE && seen.hi > k0) {  // some row of the wave sees some key of the tile
-      f32x4 S[CB][4];
+    if (EDGE && !(seen.lo < k0 + TILE && seen.hi > k0)) return;  // no row of the wave sees any of it
+    f32x4 S[CB][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 4; ++j) {
 #pragma unroll
-        for (int cb = 0; cb < CB; ++cb) S[cb][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int cb = 0; cb < CB; ++cb) S[cb][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const int row = 16 * j + col;
-          const u32x4 k = *(const u32x4*)(kb + row * HD + 8 * k_piece<HD>(row, 4 * s + g));
+      for (int s = 0; s < KS; ++s) {
+        const int row = 16 * j + col;
+        const u32x4 k = *(const u32x4*)(kb + row * HD + 8 * k_piece<HD>(row, 4 * s + g));
 #pragma unroll
-          for (int cb = 0; cb < CB; ++cb) S[cb][j] = Op<T>::mfma(k, q[cb][s], S[cb][j]);
-        }
-      }
-      const bool full = seen.full(k0);
-      u32x4 P[CB][2];
-#pragma unroll
-      for (int cb = 0; cb < CB; ++cb) {
-        const float al = next_max(m[cb], tile_scores<BIAS>(a, S[cb], r[cb], k0, g, full));
-        l[cb] = __builtin_fmaf(l[cb], al, tile_weights<BIAS>(a, S[cb], m[cb]));
-        P[cb][0] = p_operand<T>(S[cb][0], S[cb][1]);
-        P[cb][1] = p_operand<T>(S[cb][2], S[cb][3]);
-        if (__any(al != 1.f)) {
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) O[cb][nb] *= al;
-        }
-      }
-      tile_pv<T, HD, CB, NB>(O, P, vb, 0, seen.mixed(k0, LO, HI), r, k0, lane);
-    }
-    if (tn >= t_end || tn / TPC != t / TPC) {  // the chunk's last tile
-#pragma unroll
-      for (int cb = 0; cb < CB; ++cb) {
-        const float ls = rows_sum(l[cb]);
-        if (a.direct) {
-          const Fold f = fold(M[cb], L[cb], m[cb], ls);
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) Ot[cb][nb][i] = folded(f, Ot[cb][nb][i], O[cb][nb][i]);
-        } else if (r[cb].valid) {
-          const int c = t / TPC;
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) store_part<HD>(a, r[cb], c, 16 * nb + 4 * g, O[cb][nb]);
-          if (g == 0) a.ml[(r[cb].t * a.H + r[cb].h) * a.nc + c] = float2{m[cb], ls};
-        }
-        m[cb] = -INFINITY;
-        l[cb] = 0.f;
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) O[cb][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int cb = 0; cb < CB; ++cb) S[cb][j] = Op<T>::mfma(k, q[cb][s], S[cb][j]);
       }
     }
+    float mx[CB], al[CB];
+    u32x4 P[CB][2];
+    tile_scores<BIAS, CB>(a, S, mx, r, k0, g, !EDGE || seen.full(k0));
+    bool moved = false;
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+      al[cb] = next_max(m[cb], mx[cb]);
+      moved = moved || al[cb] != 1.f;
+    }
+    if (__any(moved)) {
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) {
+        l[cb] *= al[cb];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) O[cb][nb] *= al[cb];
+      }
+    }
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) tile_weights<T, BIAS>(a, S[cb], m[cb], P[cb]);
+    tile_pv<T, HD, CB, NB>(O, l, P, vb, 0, EDGE && seen.mixed(k0, LO, HI), r, k0, lane);
+  };
+  auto end_chunk = [&]() {
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+      if (a.direct) {
+        const Fold f = fold(M[cb], L[cb], m[cb], l[cb][0]);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) Ot[cb][nb][i] = folded(f, Ot[cb][nb][i], O[cb][nb][i]);
+      } else if (r[cb].valid) {
+        const int c = (unsigned)t / TPC;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) store_part<HD>(a, r[cb], c, 16 * nb + 4 * g, O[cb][nb]);
+        if (g == 0) a.ml[(r[cb].t * a.H + r[cb].h) * a.nc + c] = float2{m[cb], l[cb][0]};
+      }
+      m[cb] = -INFINITY;
+      l[cb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) O[cb][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  };
+  // Tile t out of (kb, vb) while the next one, tn, whose entries are in en, is loaded into
+  // (kn, vn), and the entries of the one after it are read; false after the last.
+  int en[LOADS];
+  const uint32_t n_in = in1 > in0 ? in1 - in0 : 0;
+  auto step = [&](const uint16_t* kb, const uint16_t* vb, uint16_t* kn, uint16_t* vn) {
+    if (tn < t_end) load(tn, en, kn, vn);
+    const int tnn = after(tn);
+    lookup(tnn, en);
+    if ((uint32_t)(t - in0) < n_in) work(std::false_type{}, kb, vb);
+    else work(std::true_type{}, kb, vb);
+    if ((t & (TPC - 1)) == TPC - 1 || tn >= t_end) end_chunk();
     if (tn >= t_end) return false;
     __builtin_amdgcn_s_waitcnt(0);  // the next tile is there,
     __syncthreads();                // and this one's buffer free
@@ -682,15 +789,15 @@ __global__ __launch_bounds__(THREADS, 2) void attn_many_kernel(AttnP a) {
     tn = tnn;
     return true;
   };
+  if (LO < HI) t = blockIdx.y == 0 ? LO / TILE : (LO / CHUNK + (int)blockIdx.y) * TPC;
   if (t < t_end) {
-    int e0[LOADS], e1[LOADS];
-    lookup(t, e0);
+    lookup(t, en);
+    load(t, en, kt0, vt0);
     tn = after(t);
-    lookup(tn, e1);
-    load(t, e0, kt0, vt0);
+    lookup(tn, en);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    while (step(kt0, vt0, kt1, vt1, e1, e0) && step(kt1, vt1, kt0, vt0, e0, e1)) {}
+    while (step(kt0, vt0, kt1, vt1) && step(kt1, vt1, kt0, vt0)) {}
   }
   if (a.direct) {
 #pragma unroll
@@ -723,7 +830,7 @@ __device__ __forceinline__ int token_segment(const AttnP& a, int64_t t, int lane
   return b;
 }
 
-// One wave per (token, head): its chunks in order, four loads ahead.
+// One wave per (token, head): its chunks in order, two groups of loads under way.
 template <class T, int HD>
 __global__ __launch_bounds__(THREADS) void attn_fold_kernel(AttnP a) {
 #pragma clang fp contract(off)
@@ -744,16 +851,19 @@ __global__ __launch_bounds__(THREADS) void attn_fold_kernel(AttnP a) {
   const float* part = a.part + row * a.nc * HD + lane * ND;
   const float2* ml = a.ml + row * a.nc;
   const int c1 = (r.hi + CHUNK - 1) / CHUNK;
-  constexpr int AHEAD = 4;
-  for (int c = r.lo / CHUNK; c < c1; c += AHEAD) {
-    vec o[AHEAD];
-    float2 x[AHEAD];
+  constexpr int AHEAD = 16;
+  const int c0 = r.lo / CHUNK;
+  vec o[2][AHEAD];
+  float2 x[2][AHEAD];
+  auto get = [&](int c, vec (&o)[AHEAD], float2 (&x)[AHEAD]) {  // past the end: the last one again, unused
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
       const int cj = c + j < c1 ? c + j : c1 - 1;
       o[j] = *(const vec*)(part + (int64_t)cj * HD);
       x[j] = ml[cj];
     }
+  };
+  auto add = [&](int c, const vec (&o)[AHEAD], const float2 (&x)[AHEAD]) {
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
       if (c + j >= c1) break;
@@ -761,6 +871,13 @@ __global__ __launch_bounds__(THREADS) void attn_fold_kernel(AttnP a) {
 #pragma unroll
       for (int i = 0; i < ND; ++i) O[i] = folded(f, O[i], o[j][i]);
     }
+  };
+  if (c0 < c1) get(c0, o[0], x[0]);
+  for (int c = c0; c < c1; c += 2 * AHEAD) {
+    if (c + AHEAD < c1) get(c + AHEAD, o[1], x[1]);
+    add(c, o[0], x[0]);
+    if (c + 2 * AHEAD < c1) get(c + 2 * AHEAD, o[0], x[0]);
+    if (c + AHEAD < c1) add(c + AHEAD, o[1], x[1]);
   }
   const float inv = 1.f / L;
   T* out = (T*)a.out + t * a.o_tok + h * a.o_head + lane * ND;
@@ -817,7 +934,7 @@ __global__ __launch_bounds__(THREADS) void attn_row_kernel(AttnP a) {
       g = page_of(a.table + (int64_t)b * a.width, a.width, a.shift, a.n_pages, key);
       float acc = 0.f;
       if (g >= 0) {
-        const T* k = (const T*)a.k + g * a.kc_page + hk * a.kc_head + (key & ((1 << a.shift) - 1)) * a.kc_slot;
+        const T* k = key_row<T>(a.k, g, key, a.shift, a.kv_page, a.kv_slot, hk * a.kv_head);
 #pragma unroll 8
         for (int d = 0; d < HD; ++d) acc = __builtin_fmaf(qs[wave][d], to_f(k[d]), acc);
       } else {
@@ -836,7 +953,7 @@ __global__ __launch_bounds__(THREADS) void attn_row_kernel(AttnP a) {
     for (int j = 0; j < TILE; ++j) {
       const int gj = pg[wave][j];
       if (gj < 0) continue;
-      const T* v = (const T*)a.v + gj * a.vc_page + hk * a.vc_head + ((k0 + j) & ((1 << a.shift) - 1)) * a.vc_slot;
+      const T* v = key_row<T>(a.v, gj, k0 + j, a.shift, a.kv_page, a.kv_slot, hk * a.kv_head);
 #pragma unroll
       for (int i = 0; i < ND; ++i) o[i] = __builtin_fmaf(ps[wave][j], to_f(v[lane + i * WAVE]), o[i]);
     }
@@ -869,7 +986,7 @@ Plan plan_of(const AltxsPagedAttnArgs* a) {
   if (p.fp32 || a->T == 0 || a->B == 0) return p;
   const int G = a->H / a->Hkv;
   p.few = a->T * G <= 16 * (int64_t)a->B;
-  const int br = p.few ? 16 : MANY;
+  const int br = p.few ? 16 : a->head_dim == 64 ? many_rows<64> : many_rows<128>;
   const int64_t slots = a->cu ? slot_count(a->T, G, br, a->B) : (int64_t)a->B * ((a->T / a->B * G + br - 1) / br);
   p.wgs = slots * a->Hkv;
   const int64_t fill = p.few ? 2048 : 512, enough = p.few ? 1024 : 384;
@@ -896,6 +1013,8 @@ static int32_t check(const AltxsPagedAttnArgs* a, const char* who) {
                 "%s: bad T, B, n_pages or table_width", who);
   ALTXS_REQUIRE(a->max_len >= 0 && a->max_len <= (int64_t)a->table_width * a->page_size,
                 "%s: max_len=%d is more than table_width * page_size", who, a->max_len);
+  for (int64_t st : {a->kv_page, a->kv_head, a->kv_slot})
+    ALTXS_REQUIRE(st >= 0 && st < (1ll << 31), "%s: a cache stride of %lld elements", who, (long long)st);
   ALTXS_REQUIRE(a->scale > 0.f && a->scale < INFINITY, "%s: scale=%g must be positive", who, a->scale);
   ALTXS_REQUIRE(a->softcap >= 0.f && a->softcap < INFINITY, "%s: softcap=%g", who, a->softcap);
   ALTXS_REQUIRE(a->window >= 0, "%s: window=%d", who, a->window);
@@ -917,8 +1036,7 @@ extern "C" int32_t altxs_paged_attn(const AltxsPagedAttnArgs* a, altxs_stream_t 
   const Plan pl = plan_of(a);
   if (!pl.fp32) {
     uintptr_t bits = (uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)a->k_cache | (uintptr_t)a->v_cache;
-    for (int64_t st : {a->q_tok, a->q_head, a->out_tok, a->out_head, a->kc_page, a->kc_head, a->kc_slot, a->vc_page, a->vc_head,
-                       a->vc_slot})
+    for (int64_t st : {a->q_tok, a->q_head, a->out_tok, a->out_head, a->kv_page, a->kv_head, a->kv_slot})
       bits |= (uintptr_t)(st * 2);
     ALTXS_REQUIRE((bits & 15) == 0, "altxs_paged_attn: rows of q, out and the caches must start at multiples of 16 bytes");
   }
@@ -931,13 +1049,12 @@ extern "C" int32_t altxs_paged_attn(const AltxsPagedAttnArgs* a, altxs_stream_t 
   p.table = a->table; p.pos = a->pos; p.cu = a->cu; p.starts = a->starts; p.prefix = a->prefix;
   p.slopes = a->slopes; p.err = a->err;
   p.T = a->T; p.n_pages = a->n_pages; p.q_tok = a->q_tok; p.q_head = a->q_head; p.o_tok = a->out_tok; p.o_head = a->out_head;
-  p.kc_page = a->kc_page; p.kc_head = a->kc_head; p.kc_slot = a->kc_slot;
-  p.vc_page = a->vc_page; p.vc_head = a->vc_head; p.vc_slot = a->vc_slot;
+  p.kv_page = (uint32_t)a->kv_page; p.kv_head = a->kv_head; p.kv_slot = (uint32_t)a->kv_slot;
   p.scale = a->scale; p.softcap = a->softcap; p.scale2 = a->scale * LOG2E;
   p.B = a->B; p.W = a->cu ? 1 : (int)(a->T / a->B); p.H = a->H; p.Hkv = a->Hkv; p.G = a->H / a->Hkv;
   p.width = a->table_width; p.shift = __builtin_ctz((unsigned)a->page_size); p.cap = a->max_len; p.window = a->window;
-  p.by_g = fast_div(p.G); p.by_hkv = fast_div(p.Hkv);
-  const int br = pl.few ? 16 : MANY;
+  p.by_g = fast_div(p.G); p.by_hkv = fast_div(p.Hkv); p.by_b = fast_div(p.B);
+  const int br = pl.few ? 16 : a->head_dim == 64 ? many_rows<64> : many_rows<128>;
   p.by_tiles = fast_div((uint32_t)(((int64_t)p.W * p.G + br - 1) / br));
   p.nc = pl.nc; p.direct = pl.split == 1;
   p.ml = (float2*)a->ws;  // then O, from a multiple of 16 bytes on
@@ -963,8 +1080,11 @@ extern "C" int32_t altxs_paged_attn(const AltxsPagedAttnArgs* a, altxs_stream_t 
     dim3 grid((unsigned)pl.wgs, (unsigned)pl.split);
     if (pl.few && bias) ALTXS_HD_GO(attn_few_kernel, true);
     else if (pl.few) ALTXS_HD_GO(attn_few_kernel, false);
-    else if (bias) ALTXS_HD_GO(attn_many_kernel, true);
-    else ALTXS_HD_GO(attn_many_kernel, false);
+    else {
+      const dim3 block(NW * WAVE);
+      if (bias) ALTXS_HD_GO(attn_many_kernel, true);
+      else ALTXS_HD_GO(attn_many_kernel, false);
+    }
     if (pl.split > 1) {
       grid = by_row;
       ALTXS_HD_GO(attn_fold_kernel);

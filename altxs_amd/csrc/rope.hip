@@ -134,16 +134,16 @@ struct AppendP {
   int32_t* err;
   int64_t T, n_pages, rope_rows;
   int64_t k_tok, k_head, v_tok, v_head, q_tok, q_head, qo_tok, qo_head;
-  int64_t kc_page, kc_head, kc_slot, vc_page, vc_head, vc_slot;
+  int64_t kv_page, kv_head, kv_slot;
   int B, Hq, Hkv, width, shift, W;  // Hq: query heads moved here (0: none); W: tokens of a segment (cu = NULL)
   Units u;
   FastDiv by_units, by_token;
   int tpb;
 };
 
-// A token's place: its rope row and its cache row's element offsets (ok = 0: skipped).
+// A token's place: its rope row and its cache row's element offset (ok = 0: skipped).
 struct Place {
-  int64_t koff, voff;
+  int64_t off;
   int32_t pos, ok;
 };
 
@@ -172,7 +172,7 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendP p) {
       c1 = c0 + p.W;
     }
     if (lane == 0) {
-      Place pl = {0, 0, 0, 0};
+      Place pl = {0, 0, 0};
       if (b < p.B) {  // rows behind the last segment belong to nobody
         const int64_t cap = (int64_t)p.width << p.shift;
         const Segment s = segment_of(c0, c1, p.pos[b], p.T, (int32_t)(cap < INT32_MAX ? cap : INT32_MAX));
@@ -185,8 +185,7 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendP p) {
             flag_err(p.err, ALTXS_EDEV_PAGE);
           } else {
             const int slot = pos & ((1 << p.shift) - 1);
-            pl.koff = g * p.kc_page + slot * p.kc_slot;
-            pl.voff = g * p.vc_page + slot * p.vc_slot;
+            pl.off = g * p.kv_page + slot * p.kv_slot;
             pl.ok = 1;
           }
           pl.pos = pos;
@@ -213,11 +212,11 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendP p) {
       dst = (T*)p.q_out + t * p.qo_tok + h * p.qo_head;
     } else if ((h -= p.Hq) < p.Hkv) {
       src = (const T*)p.k + t * p.k_tok + h * p.k_head;
-      dst = (T*)p.k_cache + pl.koff + h * p.kc_head;
+      dst = (T*)p.k_cache + pl.off + h * p.kv_head;
     } else {
       h -= p.Hkv;
       src = (const T*)p.v + t * p.v_tok + h * p.v_head;
-      dst = (T*)p.v_cache + pl.voff + h * p.vc_head;
+      dst = (T*)p.v_cache + pl.off + h * p.kv_head;
       cs = nullptr;
     }
     move_unit<T, VEC, INTER>(src, dst, cs, sn, 1.f, p.u, u);
@@ -312,6 +311,8 @@ extern "C" int32_t altxs_paged_append(const AltxsPagedAppendArgs* a, altxs_strea
   ALTXS_REQUIRE(a->T >= 0 && a->T < (1ll << 31) && a->B >= 0 && a->n_pages >= 0 && a->table_width >= 0,
                 "altxs_paged_append: bad T, B, n_pages or table_width");
   ALTXS_REQUIRE(a->rot > 0 || !a->q, "altxs_paged_append: q without a rotation");
+  for (int64_t st : {a->kv_page, a->kv_head, a->kv_slot})
+    ALTXS_REQUIRE(st >= 0 && st < (1ll << 31), "altxs_paged_append: a cache stride of %lld elements", (long long)st);
   if (a->T == 0 || a->B == 0) return ALTXS_OK;
   ALTXS_REQUIRE(a->cu || a->T % a->B == 0, "altxs_paged_append: T=%lld tokens are not B=%d equal segments",
                 (long long)a->T, a->B);
@@ -322,8 +323,8 @@ extern "C" int32_t altxs_paged_append(const AltxsPagedAppendArgs* a, altxs_strea
   const int n = 16 / elem_size(a->dtype);
   const bool inter = (a->flags & ALTXS_ROPE_INTERLEAVED) != 0;
   bool vec = dims_fit(a->head_dim, a->rot, inter, n) && fits16(a->k, n, {a->k_tok, a->k_head}) &&
-             fits16(a->v, n, {a->v_tok, a->v_head}) && fits16(a->k_cache, n, {a->kc_page, a->kc_head, a->kc_slot}) &&
-             fits16(a->v_cache, n, {a->vc_page, a->vc_head, a->vc_slot});
+             fits16(a->v, n, {a->v_tok, a->v_head}) && fits16(a->k_cache, n, {a->kv_page, a->kv_head, a->kv_slot}) &&
+             fits16(a->v_cache, n, {a->kv_page, a->kv_head, a->kv_slot});
   if (a->q) vec = vec && fits16(a->q, n, {a->q_tok, a->q_head}) && fits16(a->q_out, n, {a->q_out_tok, a->q_out_head});
   if (a->rot) vec = vec && fits16(a->cos, 4, {(int64_t)a->rot / 2}) && fits16(a->sin, 4, {(int64_t)a->rot / 2});
   AppendP p;
@@ -333,8 +334,7 @@ extern "C" int32_t altxs_paged_append(const AltxsPagedAppendArgs* a, altxs_strea
   p.T = a->T; p.n_pages = a->n_pages; p.rope_rows = a->rope_rows;
   p.k_tok = a->k_tok; p.k_head = a->k_head; p.v_tok = a->v_tok; p.v_head = a->v_head;
   p.q_tok = a->q_tok; p.q_head = a->q_head; p.qo_tok = a->q_out_tok; p.qo_head = a->q_out_head;
-  p.kc_page = a->kc_page; p.kc_head = a->kc_head; p.kc_slot = a->kc_slot;
-  p.vc_page = a->vc_page; p.vc_head = a->vc_head; p.vc_slot = a->vc_slot;
+  p.kv_page = a->kv_page; p.kv_head = a->kv_head; p.kv_slot = a->kv_slot;
   p.B = a->B; p.Hq = a->q ? a->H : 0; p.Hkv = a->Hkv; p.width = a->table_width;
   p.shift = __builtin_ctz((unsigned)a->page_size);
   p.W = a->cu ? 1 : (int)(a->T / a->B);

@@ -344,8 +344,10 @@ def _pages(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, po
            cu: torch.Tensor | None, like: torch.Tensor) -> int:
     """Check the cache's arrays; returns the number of segments."""
     dev = like.device
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
-        raise ValueError("k_cache and v_cache must be equal [n_pages, Hkv, page_size, head_dim] with contiguous rows")
+    if (k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.stride(3) != 1
+            or v_cache.stride() != k_cache.stride()):
+        raise ValueError("k_cache and v_cache must be [n_pages, Hkv, page_size, head_dim] of equal shape and strides, "
+                         "with contiguous rows")
     if k_cache.dtype != like.dtype or v_cache.dtype != like.dtype or k_cache.device != dev or v_cache.device != dev:
         raise ValueError("the caches must have the dtype and device of the heads")
     if table.dim() != 2 or table.dtype != torch.int32 or table.device != dev or not table.is_contiguous():
@@ -365,8 +367,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
                  interleaved: bool = False, err: torch.Tensor | None = None) -> torch.Tensor | None:
     """Write new keys and values k, v [T, Hkv, hd] into their segments' pages.
 
-    k_cache/v_cache [n_pages, Hkv, page_size, hd] (any strides, contiguous rows;
-    page_size a power of two, 16 to 1024), table int32 [B, width] (page ids in
+    k_cache/v_cache [n_pages, Hkv, page_size, hd] (any strides, the same for both,
+    contiguous rows; page_size a power of two, 16 to 1024), table int32 [B, width] (page ids in
     order), pos int32 [B]: new token t of segment b goes to position pos[b] + t.
     ``cu`` int32 [B + 1]: segment b's tokens are rows cu[b] to cu[b+1] (default:
     T / B each); rows from cu[B] on are left alone.  With tables ``cos``/``sin`` the
@@ -409,12 +411,12 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
                 qp, qo, qs, os_ = q.data_ptr(), result.data_ptr(), q.stride(), result.stride()
     elif q_out is not None:
         raise ValueError("q_out without cos and sin")
-    ks, vs, kc, vc = k.stride(), v.stride(), k_cache.stride(), v_cache.stride()
+    ks, vs, kc = k.stride(), v.stride(), k_cache.stride()
     a = _lib.PagedAppendArgs(k.data_ptr(), v.data_ptr(), qp, qo, k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(),
                              pos.data_ptr(), cu.data_ptr() if cu is not None else None,
                              cos.data_ptr() if rot else None, sin.data_ptr() if rot else None, _err(err, dev),
                              T, n_pages, cos.shape[0] if rot else 0, ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], os_[0], os_[1],
-                             kc[0], kc[1], kc[2], vc[0], vc[1], vc[2], B, H, Hkv, hd, page, table.shape[1], rot,
+                             kc[0], kc[1], kc[2], B, H, Hkv, hd, page, table.shape[1], rot,
                              _DT[k.dtype], _lib.ROPE_INTERLEAVED if interleaved and rot else 0)
     if Hkv:
         _launch("altxs_paged_append", a, dev)
@@ -462,13 +464,13 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
     if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (H,) or slopes.device != dev
                                or not slopes.is_contiguous()):
         raise ValueError(f"slopes must be a contiguous fp32 tensor [{H}] on {dev}")
-    qs, os_, kc, vc = q.stride(), out.stride(), k_cache.stride(), v_cache.stride()
+    qs, os_, kc = q.stride(), out.stride(), k_cache.stride()
     a = _lib.PagedAttnArgs(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), table.data_ptr(),
                            pos.data_ptr(), cu.data_ptr() if cu is not None else None,
                            _index(starts, "starts", T, dev) if starts is not None else None,
                            _index(prefix, "prefix", B, dev) if prefix is not None else None,
                            slopes.data_ptr() if slopes is not None else None, _err(err, dev), None, 0, T, n_pages,
-                           qs[0], qs[1], os_[0], os_[1], kc[0], kc[1], kc[2], vc[0], vc[1], vc[2],
+                           qs[0], qs[1], os_[0], os_[1], kc[0], kc[1], kc[2],
                            hd ** -0.5 if scale is None else scale, softcap, B, H, Hkv, hd, page, width, max_len, window,
                            _DT[q.dtype])
     n = _lib.load().altxs_paged_attn_workspace_bytes(ctypes.byref(a))

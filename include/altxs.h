@@ -601,7 +601,8 @@ int32_t altxs_pack_dense32(const float *base, const float *delta, int64_t N, int
  * two from 16 to 1024) that any segment can own:
  *   key t of segment b is row t % page_size of page table[b * table_width + t / page_size],
  *   and element d of kv head h of row s of page g is at
- *   g * *_page + h * *_head + s * *_slot + d   (strides in elements).
+ *   g * kv_page + h * kv_head + s * kv_slot + d   (strides in elements, 0 to 2^31 - 1,
+ *   the same for K and V).
  * A contiguous [n_pages, Hkv, page_size, head_dim] array is the usual layout;
  * [n_pages, page_size, Hkv, head_dim] is the same with other strides.
  * New tokens are rows of [T, heads, head_dim] arrays.  With cu = NULL every
@@ -663,7 +664,7 @@ typedef struct AltxsPagedAppendArgs {
   int32_t *err;
   int64_t T, n_pages, rope_rows;
   int64_t k_tok, k_head, v_tok, v_head, q_tok, q_head, q_out_tok, q_out_head;
-  int64_t kc_page, kc_head, kc_slot, vc_page, vc_head, vc_slot;
+  int64_t kv_page, kv_head, kv_slot;
   int32_t B, H, Hkv, head_dim, page_size, table_width, rot, dtype, flags;
   int32_t reserved;
 } AltxsPagedAppendArgs;
@@ -707,7 +708,7 @@ typedef struct AltxsPagedAttnArgs {
   int64_t ws_bytes;
   int64_t T, n_pages;
   int64_t q_tok, q_head, out_tok, out_head;
-  int64_t kc_page, kc_head, kc_slot, vc_page, vc_head, vc_slot;
+  int64_t kv_page, kv_head, kv_slot;
   float scale, softcap;   /* scale > 0; softcap >= 0 */
   int32_t B, H, Hkv, head_dim, page_size, table_width, max_len, window, dtype;
   int32_t reserved;

@@ -232,8 +232,8 @@ def test_strides():
     assert torch.equal(_bits(got), _bits(want)) and not out[:, :4].any() and not out[:, 8:].any()
     kv = torch.stack([c["k"], c["v"]], 1).to(DEV)  # K and V of a page side by side
     assert torch.equal(_bits(_run({**c, "k": kv[:, 0], "v": kv[:, 1]})), _bits(want))
-    nhd = c["k"].transpose(1, 2).contiguous().to(DEV).transpose(1, 2)
-    assert torch.equal(_bits(_run({**c, "k": nhd})), _bits(want))
+    nhd = {n: c[n].transpose(1, 2).contiguous().to(DEV).transpose(1, 2) for n in "kv"}
+    assert torch.equal(_bits(_run({**c, **nhd})), _bits(want))
     q = c["q"].to(DEV)
     assert torch.equal(_bits(_run({**c, "q": q}, out=q)), _bits(want))  # in place
 
@@ -302,7 +302,7 @@ def test_refuses():
     ok = dict(q=d["q"], k_cache=d["k"], v_cache=d["v"], table=d["table"], pos=d["pos"], cu=d["cu"])
     assert ops.paged_attn(**ok).shape == (4, 4, 64)
     i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device=DEV)  # noqa: E731
-    for kw in (dict(q=d["q"].half()), dict(q=d["q"][..., :32]), dict(k_cache=d["k"].float()), dict(v_cache=d["v"][:1]),
+    for kw in (dict(q=d["q"].half()), dict(q=d["q"][..., :32]), dict(k_cache=d["k"].float()), dict(v_cache=d["v"][:1]), dict(v_cache=d["v"].transpose(1, 2).contiguous().transpose(1, 2)),
                dict(pos=d["pos"].long()), dict(table=d["table"].long()), dict(cu=d["cu"][:2]), dict(q=d["q"][:3], cu=None),
                dict(starts=i32(3)), dict(starts=i32(4).long()), dict(prefix=i32(4)), dict(slopes=torch.zeros(3, device=DEV)),
                dict(slopes=torch.zeros(4, dtype=torch.float64, device=DEV)), dict(out=d["q"][:, :2]), dict(out=d["q"].half()),

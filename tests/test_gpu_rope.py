@@ -265,7 +265,7 @@ def test_append_layouts():
     v2.copy_(vc0)
     ops.paged_append(k, v, k2, v2, table, pos, cu=cu, cos=cos, sin=sin)
     assert torch.equal(_bits(k2), _bits(kc)) and torch.equal(_bits(v2), _bits(vc))
-    odd = torch.empty(kc.numel() + 1, dtype=kc.dtype, device=DEV)[1:].view(kc.shape)
+    odd = torch.empty(kc.numel() + 1, dtype=kc.dtype, device=DEV)[1:].view(kc.shape)  # rows off 16 bytes
     odd.copy_(kc0)
     ops.paged_append(k, v, odd, vc0, table, pos, cu=cu, cos=cos, sin=sin)
     assert torch.equal(_bits(odd), _bits(kc))

@@ -37,8 +37,8 @@ def _append(**kw):
 
 def _attn(**kw):
     a = _lib.PagedAttnArgs(T=4, n_pages=8, B=4, H=8, Hkv=8, head_dim=64, page_size=64, table_width=2, max_len=128,
-                           dtype=_lib.BF16, scale=0.125, q_tok=512, q_head=64, out_tok=512, out_head=64, kc_page=32768,
-                           kc_head=4096, kc_slot=64, vc_page=32768, vc_head=4096, vc_slot=64)
+                           dtype=_lib.BF16, scale=0.125, q_tok=512, q_head=64, out_tok=512, out_head=64, kv_page=32768,
+                           kv_head=4096, kv_slot=64)
     for n in "q k_cache v_cache out table pos".split():
         setattr(a, n, FAKE)
     for k, v in kw.items():
@@ -75,7 +75,7 @@ def test_append_refusals(kw, what):
     (dict(page_size=100), b"page_size"), (dict(max_len=129), b"max_len"), (dict(scale=0.0), b"scale"),
     (dict(scale=-1.0), b"scale"), (dict(scale=float("nan")), b"scale"), (dict(softcap=-1.0), b"softcap"),
     (dict(softcap=float("inf")), b"softcap"), (dict(window=-1), b"window"), (dict(T=5), b"equal segments"),
-    (dict(T=1 << 29), b"bad T"), (dict(q=None), b"null"), (dict(pos=None), b"null"),
+    (dict(T=1 << 29), b"bad T"), (dict(kv_slot=-64), b"stride"), (dict(kv_page=1 << 31), b"stride"), (dict(q=None), b"null"), (dict(pos=None), b"null"),
 ])
 def test_attn_refusals(kw, what):
     L = _lib.load()
