@@ -313,6 +313,8 @@ extern "C" int32_t altxs_paged_append(const AltxsPagedAppendArgs* a, altxs_strea
   ALTXS_REQUIRE(a->rot > 0 || !a->q, "altxs_paged_append: q without a rotation");
   for (int64_t st : {a->kv_page, a->kv_head, a->kv_slot})
     ALTXS_REQUIRE(st >= 0 && st < (1ll << 31), "altxs_paged_append: a cache stride of %lld elements", (long long)st);
+  ALTXS_REQUIRE((a->kv_page > 0 || a->n_pages <= 1) && (a->kv_head > 0 || a->Hkv == 1) && a->kv_slot > 0,
+                "altxs_paged_append: an expanded cache");
   if (a->T == 0 || a->B == 0) return ALTXS_OK;
   ALTXS_REQUIRE(a->cu || a->T % a->B == 0, "altxs_paged_append: T=%lld tokens are not B=%d equal segments",
                 (long long)a->T, a->B);

@@ -247,64 +247,83 @@ def rope_tables(length: int, rot: int, base: float = 1e4, *, scaling: str | None
     return tuple(torch.from_numpy((mag * f(ang)).astype(np.float32)).to(device) for f in (np.cos, np.sin))
 
 
-def _heads(t: torch.Tensor, name: str, like: torch.Tensor | None = None) -> None:
-    """A [T, heads, head_dim] device tensor whose heads are contiguous."""
-    if t.dim() != 3 or not t.is_cuda or t.stride(2) != 1:
+# Host time counts here: a decode step's rotation, append or attention runs a few
+# microseconds.  The checks below read each attribute once and build the argument
+# structure in one call; the stream comes as the handle itself (torch's public
+# current_stream builds an object for it, 1.9 us against 0.1).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _heads(t: torch.Tensor, name: str, index: int = -1, dtype=None) -> tuple:
+    """Strides of a [T, heads, head_dim] device tensor whose heads are contiguous."""
+    st = t.stride()
+    if len(st) != 3 or st[2] != 1 or not t.is_cuda:
         raise ValueError(f"{name} must be a device tensor [T, heads, head_dim] with contiguous heads")
     if t.dtype not in _DT:
         raise ValueError(f"{name} dtype {t.dtype} not supported")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+    if dtype is not None and (t.dtype != dtype or t.get_device() != index):
         raise ValueError(f"{name} must have the dtype and device of the other heads")
+    return st
 
 
-def _written(t: torch.Tensor, name: str, *reads: torch.Tensor) -> None:
-    """An output every element of which is its own, apart from or equal to what is read."""
-    for n, st in zip(t.shape, t.stride()):
-        if n > 1 and st == 0:
-            raise ValueError(f"{name} must not be expanded")
-    for x in reads:
-        if x.data_ptr() == t.data_ptr() and x.stride() == t.stride():
-            continue
-        lo, hi = t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
-        xl = x.data_ptr()
-        xh = xl + x.element_size() * (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride())))
-        if x.numel() and t.numel() and lo < xh and xl < hi:
-            raise ValueError(f"{name} must be the input itself or not overlap it")
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    lo = t.data_ptr()
+    return lo, lo + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
 
 
-def _index(t: torch.Tensor, name: str, n: int, dev) -> int:
-    if t.dtype != torch.int32 or t.device != dev or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor [{n}] on {dev}")
+def _output(t: torch.Tensor, name: str, like: torch.Tensor, *reads: torch.Tensor) -> tuple:
+    """Strides of a caller's output: ``like``'s shape, every element its own, and each tensor that
+    is read either the output itself or apart from it."""
+    st = _heads(t, name, like.get_device(), like.dtype)
+    if t.shape != like.shape:
+        raise ValueError(f"{name} must have the shape {tuple(like.shape)}")
+    if any(n > 1 and s == 0 for n, s in zip(t.shape, st)):
+        raise ValueError(f"{name} must not be expanded")
+    if t.numel():
+        lo, hi = _span(t)
+        for x in reads:
+            if x.numel() and not (x.data_ptr() == lo and x.stride() == st):
+                xl, xh = _span(x)
+                if lo < xh and xl < hi:
+                    raise ValueError(f"{name} must be the input itself or not overlap it")
+    return st
+
+
+def _index(t: torch.Tensor, name: str, n: int, index: int) -> int:
+    if t.dtype != torch.int32 or t.get_device() != index or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor [{n}] on device {index}")
     return t.data_ptr()
 
 
-def _err(err: torch.Tensor | None, dev):
+def _err(err: torch.Tensor | None, index: int):
     if err is None:
         return None
-    if err.dtype != torch.int32 or err.device != dev or err.numel() < 1:
-        raise ValueError(f"err must be an int32 tensor on {dev}")
+    if err.dtype != torch.int32 or err.get_device() != index or err.numel() < 1:
+        raise ValueError(f"err must be an int32 tensor on device {index}")
     return err.data_ptr()
 
 
-def _rot_tables(cos: torch.Tensor, sin: torch.Tensor, hd: int, dev) -> int:
-    """rot of a pair of tables [rows, rot/2]."""
-    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape != sin.shape
-            or cos.device != dev or sin.device != dev or not cos.is_contiguous() or not sin.is_contiguous()):
-        raise ValueError(f"cos and sin must be contiguous fp32 tensors [rows, rot/2] on {dev}")
-    rot = 2 * cos.shape[1]
-    if not 2 <= rot <= hd or cos.shape[0] < 1:
-        raise ValueError(f"tables of {rot} dims for heads of {hd}")
-    return rot
+def _rot_tables(cos: torch.Tensor, sin: torch.Tensor, hd: int, index: int) -> tuple[int, int]:
+    """(rows, rot) of a pair of tables [rows, rot/2]."""
+    shape = cos.shape
+    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or len(shape) != 2 or sin.shape != shape
+            or cos.get_device() != index or sin.get_device() != index or not cos.is_contiguous() or not sin.is_contiguous()):
+        raise ValueError(f"cos and sin must be contiguous fp32 tensors [rows, rot/2] on device {index}")
+    rows, half = shape
+    if not 2 <= 2 * half <= hd or rows < 1:
+        raise ValueError(f"tables of {2 * half} dims for heads of {hd}")
+    return rows, 2 * half
 
 
-def _launch(name: str, args, dev) -> None:
-    """Call ``name`` on the current stream of ``dev`` (which need not be the current device)."""
+def _launch(name: str, args, index: int) -> None:
+    """Call ``name`` on the current stream of device ``index`` (which need not be the current one)."""
     f = getattr(_lib.load(), name)
-    if dev.index == torch.cuda.current_device():
-        rc = f(ctypes.byref(args), torch.cuda.current_stream(dev).cuda_stream)
+    if index == torch.cuda.current_device():
+        rc = f(ctypes.byref(args), _raw_stream(index))
     else:
-        with torch.cuda.device(dev):
-            rc = f(ctypes.byref(args), torch.cuda.current_stream(dev).cuda_stream)
+        with torch.cuda.device(index):
+            rc = f(ctypes.byref(args), _raw_stream(index))
     if rc:
         _lib.check(rc, name)
 
@@ -321,44 +340,42 @@ def rope(x: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, sin: torch.Tenso
     outside the tables are copied unrotated and, unless it is negative
     (padding), flagged in ``err`` (int32).
     """
-    _heads(x, "x")
+    xs = _heads(x, "x")
     T, H, hd = x.shape
-    dev = x.device
-    rot = _rot_tables(cos, sin, hd, dev)
+    index = x.get_device()
+    rows, rot = _rot_tables(cos, sin, hd, index)
     if out is None:
-        out = torch.empty(T, H, hd, dtype=x.dtype, device=dev)
+        out = torch.empty((T, H, hd), dtype=x.dtype, device=x.device)
+        os_ = (H * hd, hd)
     else:
-        _heads(out, "out", x)
-        if out.shape != x.shape:
-            raise ValueError(f"out must have x's shape {tuple(x.shape)}")
-        _written(out, "out", x)
-    a = _lib.RopeArgs(x.data_ptr(), out.data_ptr(), _index(pos, "pos", T, dev), cos.data_ptr(), sin.data_ptr(),
-                      _err(err, dev), T, cos.shape[0], x.stride(0), x.stride(1), out.stride(0), out.stride(1), H, hd, rot,
-                      _DT[x.dtype], (_lib.ROPE_INTERLEAVED if interleaved else 0) | (_lib.ROPE_INVERSE if inverse else 0))
+        os_ = _output(out, "out", x, x)
+    a = _lib.RopeArgs(x.data_ptr(), out.data_ptr(), _index(pos, "pos", T, index), cos.data_ptr(), sin.data_ptr(),
+                      _err(err, index), T, rows, xs[0], xs[1], os_[0], os_[1], H, hd, rot, _DT[x.dtype],
+                      (_lib.ROPE_INTERLEAVED if interleaved else 0) | (_lib.ROPE_INVERSE if inverse else 0))
     if H:
-        _launch("altxs_rope", a, dev)
+        _launch("altxs_rope", a, index)
     return out
 
 
-def _pages(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, pos: torch.Tensor,
-           cu: torch.Tensor | None, like: torch.Tensor) -> int:
-    """Check the cache's arrays; returns the number of segments."""
-    dev = like.device
-    if (k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.stride(3) != 1
-            or v_cache.stride() != k_cache.stride()):
+def _pages(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, pos: torch.Tensor, cu: torch.Tensor | None,
+           T: int, dtype, index: int) -> tuple:
+    """Check the cache's arrays; returns (its strides, segments, table width, pos, cu)."""
+    st = k_cache.stride()
+    if len(st) != 4 or v_cache.shape != k_cache.shape or st[3] != 1 or v_cache.stride() != st:
         raise ValueError("k_cache and v_cache must be [n_pages, Hkv, page_size, head_dim] of equal shape and strides, "
                          "with contiguous rows")
-    if k_cache.dtype != like.dtype or v_cache.dtype != like.dtype or k_cache.device != dev or v_cache.device != dev:
+    if (k_cache.dtype != dtype or v_cache.dtype != dtype or k_cache.get_device() != index
+            or v_cache.get_device() != index):
         raise ValueError("the caches must have the dtype and device of the heads")
-    if table.dim() != 2 or table.dtype != torch.int32 or table.device != dev or not table.is_contiguous():
-        raise ValueError(f"table must be a contiguous int32 tensor [segments, pages] on {dev}")
-    B = table.shape[0]
-    _index(pos, "pos", B, dev)
+    if table.dim() != 2 or table.dtype != torch.int32 or table.get_device() != index or not table.is_contiguous():
+        raise ValueError(f"table must be a contiguous int32 tensor [segments, pages] on device {index}")
+    B, width = table.shape
+    pp = _index(pos, "pos", B, index)
     if cu is not None:
-        _index(cu, "cu", B + 1, dev)
-    elif B and like.shape[0] % B:
-        raise ValueError(f"{like.shape[0]} tokens are not {B} equal segments (give cu)")
-    return B
+        return st, B, width, pp, _index(cu, "cu", B + 1, index)
+    if B and T % B:
+        raise ValueError(f"{T} tokens are not {B} equal segments (give cu)")
+    return st, B, width, pp, None
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor,
@@ -377,49 +394,45 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     is returned -- a new one's rows that belong to no segment, or to one that was
     left out (``err``), are not written.  Without tables ``q`` is returned as it is.
     """
-    _heads(k, "k")
-    _heads(v, "v", k)
-    T, Hkv, hd = k.shape
-    dev = k.device
-    if v.shape != k.shape:
+    ks = _heads(k, "k")
+    T, Hkv, hd = shape = k.shape
+    index, dtype = k.get_device(), k.dtype
+    vs = _heads(v, "v", index, dtype)
+    if v.shape != shape:
         raise ValueError("k and v must have equal shapes")
-    B = _pages(k_cache, v_cache, table, pos, cu, k)
+    kv, B, width, pp, cp = _pages(k_cache, v_cache, table, pos, cu, T, dtype, index)
     n_pages, ch, page, chd = k_cache.shape
     if ch != Hkv or chd != hd:
         raise ValueError(f"caches of {ch} heads of {chd}, keys of {Hkv} of {hd}")
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin go together")
-    _written(k_cache, "k_cache", k, v)
-    _written(v_cache, "v_cache", k, v)
-    rot, H, qp, qo, qs, os_ = 0, 0, None, None, (0, 0, 0), (0, 0, 0)
+    rows = rot = H = 0
+    qp = qo = tp = sp = None
+    qs = os_ = (0, 0)
     result = q
     if cos is not None:
-        rot = _rot_tables(cos, sin, hd, dev)
+        rows, rot = _rot_tables(cos, sin, hd, index)
+        tp, sp = cos.data_ptr(), sin.data_ptr()
         if q is not None:
-            _heads(q, "q", k)
-            if q.shape[0] != T or q.shape[2] != hd:
+            qs = _heads(q, "q", index, dtype)
+            qT, H, qd = q.shape
+            if qT != T or qd != hd:
                 raise ValueError(f"q must be [{T}, heads, {hd}]")
-            result = torch.empty(q.shape, dtype=q.dtype, device=dev) if q_out is None else q_out
-            if q_out is not None:
-                _heads(q_out, "q_out", q)
-                if q_out.shape != q.shape:
-                    raise ValueError(f"q_out must have q's shape {tuple(q.shape)}")
-                _written(q_out, "q_out", q)
-                _written(q_out, "q_out", k, v)
-            H = q.shape[1]
+            if q_out is None:
+                result = torch.empty((T, H, hd), dtype=dtype, device=q.device)
+                os_ = (H * hd, hd)
+            else:
+                result, os_ = q_out, _output(q_out, "q_out", q, q, k, v)
             if H:
-                qp, qo, qs, os_ = q.data_ptr(), result.data_ptr(), q.stride(), result.stride()
+                qp, qo = q.data_ptr(), result.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out without cos and sin")
-    ks, vs, kc = k.stride(), v.stride(), k_cache.stride()
     a = _lib.PagedAppendArgs(k.data_ptr(), v.data_ptr(), qp, qo, k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(),
-                             pos.data_ptr(), cu.data_ptr() if cu is not None else None,
-                             cos.data_ptr() if rot else None, sin.data_ptr() if rot else None, _err(err, dev),
-                             T, n_pages, cos.shape[0] if rot else 0, ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], os_[0], os_[1],
-                             kc[0], kc[1], kc[2], B, H, Hkv, hd, page, table.shape[1], rot,
-                             _DT[k.dtype], _lib.ROPE_INTERLEAVED if interleaved and rot else 0)
+                             pp, cp, tp, sp, _err(err, index), T, n_pages, rows, ks[0], ks[1], vs[0], vs[1],
+                             qs[0], qs[1], os_[0], os_[1], kv[0], kv[1], kv[2], B, H, Hkv, hd, page, width, rot,
+                             _DT[dtype], _lib.ROPE_INTERLEAVED if interleaved and rot else 0)
     if Hkv:
-        _launch("altxs_paged_append", a, dev)
+        _launch("altxs_paged_append", a, index)
     return result
 
 
@@ -444,40 +457,32 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
     hold); it sizes the launch, so give it where it is known.  A row's bits
     depend on the row's own query, keys and masks alone.
     """
-    _heads(q, "q")
+    qs = _heads(q, "q")
     T, H, hd = q.shape
-    dev = q.device
-    B = _pages(k_cache, v_cache, table, pos, cu, q)
+    index, dtype = q.get_device(), q.dtype
+    kv, B, width, pp, cp = _pages(k_cache, v_cache, table, pos, cu, T, dtype, index)
     n_pages, Hkv, page, chd = k_cache.shape
     if chd != hd:
         raise ValueError(f"caches of heads of {chd}, queries of {hd}")
-    width = table.shape[1]
-    max_len = width * page if max_len is None else int(max_len)
     if out is None:
-        out = torch.empty(T, H, hd, dtype=q.dtype, device=dev)
+        out = torch.empty((T, H, hd), dtype=dtype, device=q.device)
+        os_ = (H * hd, hd)
     else:
-        _heads(out, "out", q)
-        if out.shape != q.shape:
-            raise ValueError(f"out must have q's shape {tuple(q.shape)}")
-        _written(out, "out", q)
-        _written(out, "out", k_cache, v_cache)
-    if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (H,) or slopes.device != dev
+        os_ = _output(out, "out", q, q)
+    if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (H,) or slopes.get_device() != index
                                or not slopes.is_contiguous()):
-        raise ValueError(f"slopes must be a contiguous fp32 tensor [{H}] on {dev}")
-    qs, os_, kc = q.stride(), out.stride(), k_cache.stride()
-    a = _lib.PagedAttnArgs(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), table.data_ptr(),
-                           pos.data_ptr(), cu.data_ptr() if cu is not None else None,
-                           _index(starts, "starts", T, dev) if starts is not None else None,
-                           _index(prefix, "prefix", B, dev) if prefix is not None else None,
-                           slopes.data_ptr() if slopes is not None else None, _err(err, dev), None, 0, T, n_pages,
-                           qs[0], qs[1], os_[0], os_[1], kc[0], kc[1], kc[2],
-                           hd ** -0.5 if scale is None else scale, softcap, B, H, Hkv, hd, page, width, max_len, window,
-                           _DT[q.dtype])
+        raise ValueError(f"slopes must be a contiguous fp32 tensor [{H}] on device {index}")
+    a = _lib.PagedAttnArgs(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), table.data_ptr(), pp, cp,
+                           _index(starts, "starts", T, index) if starts is not None else None,
+                           _index(prefix, "prefix", B, index) if prefix is not None else None,
+                           slopes.data_ptr() if slopes is not None else None, _err(err, index), None, 0, T, n_pages,
+                           qs[0], qs[1], os_[0], os_[1], kv[0], kv[1], kv[2], hd ** -0.5 if scale is None else scale, softcap,
+                           B, H, Hkv, hd, page, width, width * page if max_len is None else max_len, window, _DT[dtype])
     n = _lib.load().altxs_paged_attn_workspace_bytes(ctypes.byref(a))
-    if n < 0:
-        _lib.check(int(n), "altxs_paged_attn")
     if n:
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        if n < 0:
+            _lib.check(int(n), "altxs_paged_attn")
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
         a.ws, a.ws_bytes = ws.data_ptr(), n
-    _launch("altxs_paged_attn", a, dev)
+    _launch("altxs_paged_attn", a, index)
     return out

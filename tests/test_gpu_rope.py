@@ -313,9 +313,11 @@ def test_append_refuses():
                dict(v_cache=vc[:, :, :8]), dict(table=table.long()), dict(table=table[0]), dict(table=table.t()),
                dict(pos=pos.long()), dict(pos=pos[:1]), dict(cu=cu[:2]), dict(cos=None), dict(q=q[:1]), dict(q=q.half()),
                dict(q_out=q[:, :2]), dict(q_out=k[:, :1].expand(4, 4, 64)), dict(cos=None, sin=None, q_out=q),
-               dict(k=k[:3], v=v[:3], q=q[:3], cu=None), dict(k_cache=kc[:1].expand(*kc.shape)), dict(pos=pos.cpu())):
+               dict(k=k[:3], v=v[:3], q=q[:3], cu=None), dict(pos=pos.cpu())):
         with pytest.raises(ValueError):
             ops.paged_append(**{**ok, **kw})
+    with pytest.raises(RuntimeError, match="expanded"):
+        ops.paged_append(k, v, kc[:1].expand(*kc.shape), vc[:1].expand(*vc.shape), table, pos, cu=cu)
     with pytest.raises(RuntimeError, match="page_size"):
         ops.paged_append(k, v, kc[:, :, :12], vc[:, :, :12], table, pos, cu=cu)
     before = kc.clone()

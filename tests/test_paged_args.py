@@ -27,7 +27,7 @@ def _rope(**kw):
 
 def _append(**kw):
     a = _lib.PagedAppendArgs(T=4, n_pages=8, rope_rows=64, B=4, H=8, Hkv=8, head_dim=64, page_size=64, table_width=2, rot=16,
-                             dtype=_lib.BF16)
+                             dtype=_lib.BF16, kv_page=32768, kv_head=4096, kv_slot=64)
     for n in "k v q q_out k_cache v_cache table pos cos sin".split():
         setattr(a, n, FAKE)
     for k, v in kw.items():
@@ -63,6 +63,7 @@ def test_rope_refusals(kw, what):
     (dict(Hkv=0), b"Hkv"), (dict(H=0), b"H="), (dict(page_size=48), b"page_size"), (dict(page_size=8), b"page_size"),
     (dict(T=5), b"equal segments"), (dict(k=None), b"null"), (dict(q_out=None), b"null"), (dict(table=None), b"null"),
     (dict(sin=None), b"null"), (dict(rope_rows=0), b"rope_rows"), (dict(B=-1), b"bad T"), (dict(T=1 << 31), b"bad T"),
+    (dict(kv_slot=-64), b"stride"), (dict(kv_page=1 << 31), b"stride"), (dict(kv_page=0), b"expanded"), (dict(kv_head=0), b"expanded"),
 ])
 def test_append_refusals(kw, what):
     L = _lib.load()
