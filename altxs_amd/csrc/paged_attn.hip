@@ -126,11 +126,11 @@ __device__ __forceinline__ RowTile find_tile(const AttnP& a, int slot, int br, i
 
 // One query row as a lane's column sees it.
 struct Row {
-  int lo, hi, p;      // rows past the segment's last: everything is let through, nothing stored
+  int lo, hi, p;      // rows past the segment's last, and rows that see nothing, let everything through
   float slope2;       // slope * log2(e)
   int64_t t;          // token
   int h;              // query head
-  bool valid, empty;  // empty: a valid row that sees nothing
+  bool valid, empty;  // not valid: past the last, nothing is stored; empty: sees nothing, zeros are stored
 };
 
 __device__ __forceinline__ Row row_of(const AttnP& a, const RowTile& tile, int hk, int r) {
@@ -145,8 +145,8 @@ __device__ __forceinline__ Row row_of(const AttnP& a, const RowTile& tile, int h
   if (tile.s.ok)
     k = keys_seen(o.p, tile.s.pos + tile.s.n, a.window, a.starts ? a.starts[o.t] : 0, a.prefix ? a.prefix[tile.b] : 0);
   o.empty = o.valid && k.lo >= k.hi;
-  o.lo = o.valid ? k.lo : 0;
-  o.hi = o.valid ? k.hi : INT32_MAX;
+  o.lo = o.valid && !o.empty ? k.lo : 0;
+  o.hi = o.valid && !o.empty ? k.hi : INT32_MAX;
   o.slope2 = a.slopes ? a.slopes[o.h] * LOG2E : 0.f;
   return o;
 }
@@ -161,8 +161,8 @@ __device__ __forceinline__ int row16_imin(int v) {
 }
 __device__ __forceinline__ int row16_imax(int v) { return -row16_imin(-v); }
 
-// What a set of rows sees: the union [lo, hi) and what all of them see, [clo, chi)
-// (rows that see nothing make it empty).
+// What a set of rows sees: the union [lo, hi) and what all of them see, [clo, chi); rows
+// that see nothing do not count.
 struct Seen {
   int lo, hi, clo, chi;
   __device__ bool full(int k0) const { return clo <= k0 && chi >= k0 + TILE; }
@@ -176,8 +176,8 @@ __device__ __forceinline__ Seen seen_by(const Row& r) {
   const bool some = r.valid && !r.empty;
   s.lo = row16_imin(some ? r.lo : INT32_MAX);
   s.hi = row16_imax(some ? r.hi : 0);
-  s.clo = row16_imax(!r.valid ? 0 : r.empty ? INT32_MAX : r.lo);
-  s.chi = row16_imin(!r.valid ? INT32_MAX : r.empty ? 0 : r.hi);
+  s.clo = row16_imax(r.lo);
+  s.chi = row16_imin(r.hi);
   return s;
 }
 __device__ __forceinline__ Seen both(const Seen a, const Seen b) {
@@ -632,7 +632,7 @@ __global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
   for (int w = 0; w < NW; ++w) all = both(all, Seen{range[0][w], range[1][w], range[2][w], range[3][w]});
   const int LO = __builtin_amdgcn_readfirstlane(all.lo), HI = __builtin_amdgcn_readfirstlane(all.hi);
   // tiles [in0, in1) are seen whole by every row of the workgroup
-  const int in0 = (__builtin_amdgcn_readfirstlane(all.clo < INT32_MAX - TILE ? all.clo : INT32_MAX - TILE) + TILE - 1) / TILE;
+  const int in0 = (__builtin_amdgcn_readfirstlane(all.clo) + TILE - 1) / TILE;
   const int in1 = __builtin_amdgcn_readfirstlane(all.chi) / TILE;
 
   float m[CB], M[CB], L[CB];
@@ -830,11 +830,14 @@ __device__ __forceinline__ int token_segment(const AttnP& a, int64_t t, int lane
   return b;
 }
 
-// One wave per (token, head): its chunks in order, two groups of loads under way.
+// One wave per (token, head): a dim (or two) per lane for O, and for each 64 chunks a
+// chunk per lane for the factors -- the running maximum is a prefix maximum, so a
+// scan over the lanes gives the values of fold() for all of them at once.  O is
+// folded in order with the chunks' loads two groups ahead.
 template <class T, int HD>
 __global__ __launch_bounds__(THREADS) void attn_fold_kernel(AttnP a) {
 #pragma clang fp contract(off)
-  constexpr int ND = HD / WAVE;
+  constexpr int ND = HD / WAVE, AHEAD = 16;
   typedef __attribute__((ext_vector_type(ND))) float vec;
   const int wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE;
   const int64_t row = (int64_t)blockIdx.x * WAVES + wave;
@@ -846,38 +849,47 @@ __global__ __launch_bounds__(THREADS) void attn_fold_kernel(AttnP a) {
   if (b < 0 || t < s.t0 || t >= s.t0 + s.n) return;
   Range r = {0, 0};
   if (s.ok) r = keys_seen(s.pos + (int)(t - s.t0), s.pos + s.n, a.window, a.starts ? a.starts[t] : 0, a.prefix ? a.prefix[b] : 0);
-  float M = -INFINITY, L = 0.f;
-  vec O = 0.f;
   const float* part = a.part + row * a.nc * HD + lane * ND;
   const float2* ml = a.ml + row * a.nc;
-  const int c1 = (r.hi + CHUNK - 1) / CHUNK;
-  constexpr int AHEAD = 16;
-  const int c0 = r.lo / CHUNK;
+  const int c0 = __builtin_amdgcn_readfirstlane(r.lo / CHUNK), c1 = __builtin_amdgcn_readfirstlane((r.hi + CHUNK - 1) / CHUNK);
+  float M = -INFINITY, L = 0.f;
+  vec O = 0.f;
   vec o[2][AHEAD];
-  float2 x[2][AHEAD];
-  auto get = [&](int c, vec (&o)[AHEAD], float2 (&x)[AHEAD]) {  // past the end: the last one again, unused
+  auto get = [&](int c, vec (&o)[AHEAD]) {  // past the end: the last one again, unused
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      const int cj = c + j < c1 ? c + j : c1 - 1;
-      o[j] = *(const vec*)(part + (int64_t)cj * HD);
-      x[j] = ml[cj];
-    }
+    for (int j = 0; j < AHEAD; ++j) o[j] = *(const vec*)(part + (int64_t)(c + j < c1 ? c + j : c1 - 1) * HD);
   };
-  auto add = [&](int c, const vec (&o)[AHEAD], const float2 (&x)[AHEAD]) {
+  for (int c = c0; c < c1; c += WAVE) {
+    const float2 x = c + lane < c1 ? ml[c + lane] : float2{-INFINITY, 0.f};
+    get(c, o[0]);
+    float mx = fmaxf(x.x, M);  // maximum of the chunks up to the lane's
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      if (c + j >= c1) break;
-      const Fold f = fold(M, L, x[j].x, x[j].y);
-#pragma unroll
-      for (int i = 0; i < ND; ++i) O[i] = folded(f, O[i], o[j][i]);
+    for (int d = 1; d < WAVE; d *= 2) {
+      const float up = __shfl_up(mx, d, WAVE);
+      mx = fmaxf(mx, lane >= d ? up : -INFINITY);
     }
-  };
-  if (c0 < c1) get(c0, o[0], x[0]);
-  for (int c = c0; c < c1; c += 2 * AHEAD) {
-    if (c + AHEAD < c1) get(c + AHEAD, o[1], x[1]);
-    add(c, o[0], x[0]);
-    if (c + 2 * AHEAD < c1) get(c + 2 * AHEAD, o[0], x[0]);
-    if (c + AHEAD < c1) add(c + AHEAD, o[1], x[1]);
+    const float up = __shfl_up(mx, 1, WAVE), before = lane ? up : M;
+    const float fa = before == mx ? 1.f : __builtin_amdgcn_exp2f(before - mx);
+    const float fb = x.x == mx ? 1.f : __builtin_amdgcn_exp2f(x.x - mx);
+    auto add = [&](int j0, const vec (&o)[AHEAD]) {
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const float fj = lane_f(fa, j0 + j), gj = lane_f(fb, j0 + j), lj = lane_f(x.y, j0 + j);
+        if (c + j0 + j < c1) {
+          L = __builtin_fmaf(lj, gj, L * fj);
+#pragma unroll
+          for (int i = 0; i < ND; ++i) O[i] = __builtin_fmaf(o[j][i], gj, O[i] * fj);
+        }
+      }
+    };
+#pragma unroll
+    for (int j0 = 0; j0 < WAVE; j0 += 2 * AHEAD) {
+      if (c + j0 + AHEAD < c1) get(c + j0 + AHEAD, o[1]);
+      add(j0, o[0]);
+      if (c + j0 + 2 * AHEAD < c1 && j0 + 2 * AHEAD < WAVE) get(c + j0 + 2 * AHEAD, o[0]);
+      if (c + j0 + AHEAD < c1) add(j0 + AHEAD, o[1]);
+    }
+    M = lane_f(mx, WAVE - 1);
   }
   const float inv = 1.f / L;
   T* out = (T*)a.out + t * a.o_tok + h * a.o_head + lane * ND;
@@ -989,7 +1001,7 @@ Plan plan_of(const AltxsPagedAttnArgs* a) {
   const int br = p.few ? 16 : a->head_dim == 64 ? many_rows<64> : many_rows<128>;
   const int64_t slots = a->cu ? slot_count(a->T, G, br, a->B) : (int64_t)a->B * ((a->T / a->B * G + br - 1) / br);
   p.wgs = slots * a->Hkv;
-  const int64_t fill = p.few ? 2048 : 512, enough = p.few ? 1024 : 384;
+  const int64_t fill = p.few ? 2048 : 512, enough = 384;
   if (p.wgs < enough) {
     const int64_t z = (fill + p.wgs - 1) / p.wgs;
     p.split = (int)(z < p.nc ? z : p.nc);
