@@ -76,4 +76,30 @@ ALTXS_HD int32_t page_of(const int32_t* row, int32_t width, int32_t shift, int64
   return g < 0 || g >= n_pages ? -1 : g;
 }
 
+#if defined(__HIPCC__)
+// The segment of token t, asked by a whole wave: 64 segments per step, each lane with
+// one's bounds and position (so nothing is read again once it is found); -1: the token
+// belongs to nobody.  cu = NULL: every segment has W tokens.
+__device__ __forceinline__ int token_segment(const int32_t* cu, const int32_t* pos, int B, int W, int64_t t, int64_t T, int cap,
+                                             int lane, Segment& s) {
+  if (!cu) {
+    const int b = (int)(t / W);
+    s = segment_of(b * W, b * W + W, pos[b], T, cap);
+    return b;
+  }
+  for (int i = 0; i < B; i += 64) {
+    const int j = i + lane < B ? i + lane : B - 1;
+    const int c0 = cu[j], c1 = cu[j + 1], p = pos[j];
+    const uint64_t later = __ballot(i + lane < B && c1 > t);
+    if (later) {
+      const int l = __builtin_ctzll(later);
+      s = segment_of(__builtin_amdgcn_readlane(c0, l), __builtin_amdgcn_readlane(c1, l), __builtin_amdgcn_readlane(p, l), T, cap);
+      return i + l;
+    }
+  }
+  s = Segment{0, 0, 0, 0};
+  return -1;
+}
+#endif
+
 }  // namespace altxs_paged

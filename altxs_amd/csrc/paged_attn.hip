@@ -812,24 +812,6 @@ __global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
 
 // ---- folding the chunks' partial results ---------------------------------------
 
-// The segment of token t (a whole wave asks): -1 behind the last one.
-__device__ __forceinline__ int token_segment(const AttnP& a, int64_t t, int lane, Segment& s) {
-  int b, c0, c1;
-  if (a.cu) {
-    b = 0;
-    for (int i = 0; i < a.B; i += WAVE) b += __builtin_popcountll(__ballot(i + lane < a.B && a.cu[i + lane + 1] <= t));
-    if (b >= a.B) return -1;
-    c0 = a.cu[b];
-    c1 = a.cu[b + 1];
-  } else {
-    b = (int)(t / a.W);
-    c0 = b * a.W;
-    c1 = c0 + a.W;
-  }
-  s = segment_of(c0, c1, a.pos[b], a.T, a.cap);
-  return b;
-}
-
 // One wave per (token, head): a dim (or two) per lane for O, and for each 64 chunks a
 // chunk per lane for the factors -- the running maximum is a prefix maximum, so a
 // scan over the lanes gives the values of fold() for all of them at once.  O is
@@ -845,7 +827,7 @@ __global__ __launch_bounds__(THREADS) void attn_fold_kernel(AttnP a) {
   const int64_t t = row / a.H;
   const int h = (int)(row - t * a.H);
   Segment s;
-  const int b = token_segment(a, t, lane, s);
+  const int b = token_segment(a.cu, a.pos, a.B, a.W, t, a.T, a.cap, lane, s);
   if (b < 0 || t < s.t0 || t >= s.t0 + s.n) return;
   Range r = {0, 0};
   if (s.ok) r = keys_seen(s.pos + (int)(t - s.t0), s.pos + s.n, a.window, a.starts ? a.starts[t] : 0, a.prefix ? a.prefix[b] : 0);
@@ -926,7 +908,7 @@ __global__ __launch_bounds__(THREADS) void attn_row_kernel(AttnP a) {
   const int64_t t = row / a.H;
   const int h = (int)(row - t * a.H), hk = h / a.G;
   Segment s;
-  const int b = token_segment(a, t, lane, s);
+  const int b = token_segment(a.cu, a.pos, a.B, a.W, t, a.T, a.cap, lane, s);
   if (b < 0) return;  // behind the last segment
   Range r = {0, 0};
   const int p = s.pos + (int)(t - s.t0);

@@ -27,6 +27,13 @@ __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__bf16 x) { return (float)x; }
 __device__ __forceinline__ float to_f(_Float16 x) { return (float)x; }
 
+// fp32 -> T in a rounding of its own: fused into the product before it (v_fma_mixlo_f16),
+// it would give a kernel's fp16 rows other bits than another's.
+template <class T> __device__ __forceinline__ T rounded(float x) {
+  if constexpr (std::is_same_v<T, _Float16>) asm("" : "+v"(x));
+  return (T)x;
+}
+
 // How a head's row is cut into units.
 struct Units {
   int nrot;   // rotated units
@@ -34,64 +41,61 @@ struct Units {
   int half;   // rot / 2
 };
 
-// One unit of one head row.  cs/sn: the position's table rows (NULL: copy).
-template <class T, bool VEC, bool INTER>
-__device__ __forceinline__ void move_unit(const T* src, T* dst, const float* cs, const float* sn, float sgn,
-                                          const Units u, int i) {
+// One unit of one head row on its way: get() reads it, put() rotates and writes it.  A
+// kernel reads first and finds the position and the place meanwhile: both cost a
+// memory latency or three.  cs/sn: the position's table rows (NULL: copy).
+template <class T, bool VEC, bool INTER> struct Unit {
+  static constexpr int N = VEC ? 16 / (int)sizeof(T) : 1;  // elements of a vector
+  static constexpr bool PAIR = !VEC || !INTER;             // firsts and seconds are two accesses
+  std::conditional_t<VEC, Vec<T>, T> x, y;
+  T* dst;
+  const float *cs, *sn;
+  int i;  // unit of its head
+
+  __device__ __forceinline__ int first(const Units& u) const {
+    return i >= u.nrot ? 2 * u.half + (i - u.nrot) * N : VEC || !INTER ? i * N : 2 * i;
+  }
+  __device__ __forceinline__ int second(const Units& u) const { return INTER ? 2 * i + 1 : i * N + u.half; }
+
+  __device__ __forceinline__ void get(const T* src, const Units& u) {
+    using V = decltype(x);
+    x = *(const V*)(src + first(u));
+    if (PAIR && i < u.nrot) y = *(const V*)(src + second(u));
+  }
+  __device__ __forceinline__ void put(const Units& u, float sgn) {
 #pragma clang fp contract(off)
-  constexpr int N = VEC ? 16 / (int)sizeof(T) : 1;
-  if (i >= u.nrot) {  // unrotated dims
-    const int d = 2 * u.half + (i - u.nrot) * N;
-    if constexpr (VEC) *(Vec<T>*)(dst + d) = *(const Vec<T>*)(src + d);
-    else dst[d] = src[d];
-    return;
+    using V = decltype(x);
+    if (i < u.nrot && cs) {
+      if constexpr (VEC && INTER) {
+        typedef __attribute__((ext_vector_type(N / 2))) float pairs_t;
+        const pairs_t c = *(const pairs_t*)(cs + i * N / 2), s = sgn * *(const pairs_t*)(sn + i * N / 2);
+#pragma unroll
+        for (int j = 0; j < N / 2; ++j) {
+          const float a = to_f(x.v[2 * j]), b = to_f(x.v[2 * j + 1]);
+          x.v[2 * j] = rounded<T>(__builtin_fmaf(b, s[j], a * c[j]));
+          x.v[2 * j + 1] = rounded<T>(__builtin_fmaf(-a, s[j], b * c[j]));
+        }
+      } else if constexpr (VEC) {
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+          const f32x4 c = *(const f32x4*)(cs + i * N + j), s = sgn * *(const f32x4*)(sn + i * N + j);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float a = to_f(x.v[j + k]), b = to_f(y.v[j + k]);
+            x.v[j + k] = rounded<T>(__builtin_fmaf(b, s[k], a * c[k]));
+            y.v[j + k] = rounded<T>(__builtin_fmaf(-a, s[k], b * c[k]));
+          }
+        }
+      } else {
+        const float a = to_f(x), b = to_f(y), c = cs[i], s = sgn * sn[i];
+        x = rounded<T>(__builtin_fmaf(b, s, a * c));
+        y = rounded<T>(__builtin_fmaf(-a, s, b * c));
+      }
+    }
+    *(V*)(dst + first(u)) = x;
+    if (PAIR && i < u.nrot) *(V*)(dst + second(u)) = y;
   }
-  if constexpr (VEC && INTER) {
-    const int d = i * N;
-    Vec<T> x = *(const Vec<T>*)(src + d);
-    if (cs) {
-      typedef __attribute__((ext_vector_type(N / 2))) float pairs_t;
-      const pairs_t c = *(const pairs_t*)(cs + d / 2), s = sgn * *(const pairs_t*)(sn + d / 2);
-#pragma unroll
-      for (int j = 0; j < N / 2; ++j) {
-        const float a = to_f(x.v[2 * j]), b = to_f(x.v[2 * j + 1]);
-        x.v[2 * j] = (T)__builtin_fmaf(b, s[j], a * c[j]);
-        x.v[2 * j + 1] = (T)__builtin_fmaf(-a, s[j], b * c[j]);
-      }
-    }
-    *(Vec<T>*)(dst + d) = x;
-  } else if constexpr (VEC) {
-    const int d = i * N;
-    Vec<T> x = *(const Vec<T>*)(src + d), y = *(const Vec<T>*)(src + u.half + d);
-    if (cs) {
-      float c[N], s[N];
-#pragma unroll
-      for (int j = 0; j < N; j += 4) {
-        *(f32x4*)(c + j) = *(const f32x4*)(cs + d + j);
-        *(f32x4*)(s + j) = *(const f32x4*)(sn + d + j);
-      }
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float a = to_f(x.v[j]), b = to_f(y.v[j]), sj = sgn * s[j];
-        x.v[j] = (T)__builtin_fmaf(b, sj, a * c[j]);
-        y.v[j] = (T)__builtin_fmaf(-a, sj, b * c[j]);
-      }
-    }
-    *(Vec<T>*)(dst + d) = x;
-    *(Vec<T>*)(dst + u.half + d) = y;
-  } else {
-    const int d0 = INTER ? 2 * i : i, d1 = INTER ? d0 + 1 : i + u.half;
-    const float a = to_f(src[d0]), b = to_f(src[d1]);
-    if (cs) {
-      const float c = cs[i], s = sgn * sn[i];
-      dst[d0] = (T)__builtin_fmaf(b, s, a * c);
-      dst[d1] = (T)__builtin_fmaf(-a, s, b * c);
-    } else {
-      dst[d0] = (T)a;
-      dst[d1] = (T)b;
-    }
-  }
-}
+};
 
 struct RopeP {
   const void* x;
@@ -114,15 +118,18 @@ __global__ __launch_bounds__(THREADS) void rope_kernel(RopeP p) {
   const int n = nt * (int)p.by_token.d;
   for (int i = threadIdx.x; i < n; i += THREADS) {
     const uint32_t tl = div_by(i, p.by_token), j = i - tl * p.by_token.d;
-    const uint32_t h = div_by(j, p.by_units), u = j - h * p.by_units.d;
+    const uint32_t h = div_by(j, p.by_units);
     const int64_t t = t0 + tl;
+    Unit<T, VEC, INTER> m;
+    m.i = j - h * p.by_units.d;
+    m.get((const T*)p.x + t * p.x_tok + h * p.x_head, p.u);
     const int32_t pos = p.pos[t];
     const bool ok = pos >= 0 && pos < p.rows;
     if (!ok && pos >= 0 && j == 0) flag_err(p.err, ALTXS_EDEV_POS);
-    const float* cs = ok ? p.cos + (int64_t)pos * p.u.half : nullptr;
-    const float* sn = ok ? p.sin + (int64_t)pos * p.u.half : nullptr;
-    move_unit<T, VEC, INTER>((const T*)p.x + t * p.x_tok + h * p.x_head, (T*)p.out + t * p.out_tok + h * p.out_head, cs, sn,
-                             p.sgn, p.u, u);
+    m.cs = ok ? p.cos + (int64_t)pos * p.u.half : nullptr;
+    m.sn = p.sin + (ok ? (int64_t)pos * p.u.half : 0);
+    m.dst = (T*)p.out + t * p.out_tok + h * p.out_head;
+    m.put(p.u, p.sgn);
   }
 }
 
@@ -149,77 +156,62 @@ struct Place {
 
 constexpr int MAX_TPB = 64;
 
-// The workgroup's tokens find their segments first, a wave per token: the number
-// of entries cu[1..B] at or below the token, 64 of them per step.
+// The tokens' places are found by a wave each while the first units are read.
 template <class T, bool VEC, bool INTER>
 __global__ __launch_bounds__(THREADS) void append_kernel(AppendP p) {
   __shared__ Place place[MAX_TPB];
   const int64_t t0 = (int64_t)blockIdx.x * p.tpb;
   const int nt = (int)(p.T - t0 < p.tpb ? p.T - t0 : p.tpb);
   const int wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE;
-  for (int tl = wave; tl < nt; tl += THREADS / WAVE) {
+  const int n = nt * (int)p.by_token.d;
+  int tl = 0, h = 0;
+  Unit<T, VEC, INTER> m;
+  auto get = [&](int i) {
+    tl = (int)div_by(i, p.by_token);
+    const uint32_t j = i - tl * p.by_token.d;
+    h = (int)div_by(j, p.by_units);
+    m.i = (int)(j - h * p.by_units.d);
     const int64_t t = t0 + tl;
-    int b, c0, c1;
-    if (p.cu) {
-      b = 0;
-      for (int i = 0; i < p.B; i += WAVE)
-        b += __builtin_popcountll(__ballot(i + lane < p.B && p.cu[i + lane + 1] <= t));
-      c0 = b < p.B ? p.cu[b] : 0;
-      c1 = b < p.B ? p.cu[b + 1] : 0;
-    } else {
-      b = (int)(t / p.W);
-      c0 = b * p.W;
-      c1 = c0 + p.W;
-    }
+    const T* src = h < p.Hq           ? (const T*)p.q + t * p.q_tok + h * p.q_head
+                   : h < p.Hq + p.Hkv ? (const T*)p.k + t * p.k_tok + (h - p.Hq) * p.k_head
+                                      : (const T*)p.v + t * p.v_tok + (h - p.Hq - p.Hkv) * p.v_head;
+    m.get(src, p.u);
+  };
+  auto put = [&]() {
+    const Place pl = place[tl];
+    if (!pl.ok) return;
+    const bool is_v = h >= p.Hq + p.Hkv;
+    m.dst = h < p.Hq ? (T*)p.q_out + (t0 + tl) * p.qo_tok + h * p.qo_head
+            : is_v   ? (T*)p.v_cache + pl.off + (h - p.Hq - p.Hkv) * p.kv_head
+                     : (T*)p.k_cache + pl.off + (h - p.Hq) * p.kv_head;
+    m.cs = p.cos && !is_v ? p.cos + (int64_t)pl.pos * p.u.half : nullptr;
+    m.sn = p.sin + (int64_t)pl.pos * p.u.half;
+    m.put(p.u, 1.f);
+  };
+  if ((int)threadIdx.x < n) get(threadIdx.x);
+  for (int i = wave; i < nt; i += THREADS / WAVE) {
+    const int64_t t = t0 + i, cap = (int64_t)p.width << p.shift;
+    Segment s;
+    const int b = token_segment(p.cu, p.pos, p.B, p.W, t, p.T, (int)(cap < INT32_MAX ? cap : INT32_MAX), lane, s);
     if (lane == 0) {
       Place pl = {0, 0, 0};
-      if (b < p.B) {  // rows behind the last segment belong to nobody
-        const int64_t cap = (int64_t)p.width << p.shift;
-        const Segment s = segment_of(c0, c1, p.pos[b], p.T, (int32_t)(cap < INT32_MAX ? cap : INT32_MAX));
+      if (b >= 0) {  // rows behind the last segment belong to nobody
         const int32_t pos = s.pos + (int32_t)(t - s.t0);
         if (!s.ok || t < s.t0 || t >= s.t0 + s.n || (p.cos && pos >= p.rope_rows)) {
           flag_err(p.err, ALTXS_EDEV_POS);
         } else {
           const int32_t g = page_of(p.table + (int64_t)b * p.width, p.width, p.shift, p.n_pages, pos);
-          if (g < 0) {
-            flag_err(p.err, ALTXS_EDEV_PAGE);
-          } else {
-            const int slot = pos & ((1 << p.shift) - 1);
-            pl.off = g * p.kv_page + slot * p.kv_slot;
-            pl.ok = 1;
-          }
-          pl.pos = pos;
+          if (g < 0) flag_err(p.err, ALTXS_EDEV_PAGE);
+          else pl = Place{g * p.kv_page + (pos & ((1 << p.shift) - 1)) * p.kv_slot, pos, 1};
         }
       }
-      place[tl] = pl;
+      place[i] = pl;
     }
   }
   __syncthreads();
-  const int n = nt * (int)p.by_token.d;
-  for (int i = threadIdx.x; i < n; i += THREADS) {
-    const uint32_t tl = div_by(i, p.by_token), j = i - tl * p.by_token.d;
-    int h = (int)div_by(j, p.by_units);
-    const int u = (int)(j - h * p.by_units.d);
-    const Place pl = place[tl];
-    if (!pl.ok) continue;
-    const int64_t t = t0 + tl;
-    const float* cs = p.cos ? p.cos + (int64_t)pl.pos * p.u.half : nullptr;
-    const float* sn = p.cos ? p.sin + (int64_t)pl.pos * p.u.half : nullptr;
-    const T* src;
-    T* dst;
-    if (h < p.Hq) {
-      src = (const T*)p.q + t * p.q_tok + h * p.q_head;
-      dst = (T*)p.q_out + t * p.qo_tok + h * p.qo_head;
-    } else if ((h -= p.Hq) < p.Hkv) {
-      src = (const T*)p.k + t * p.k_tok + h * p.k_head;
-      dst = (T*)p.k_cache + pl.off + h * p.kv_head;
-    } else {
-      h -= p.Hkv;
-      src = (const T*)p.v + t * p.v_tok + h * p.v_head;
-      dst = (T*)p.v_cache + pl.off + h * p.kv_head;
-      cs = nullptr;
-    }
-    move_unit<T, VEC, INTER>(src, dst, cs, sn, 1.f, p.u, u);
+  for (int i = threadIdx.x; i < n;) {
+    put();
+    if ((i += THREADS) < n) get(i);
   }
 }
 

@@ -48,7 +48,7 @@ def test_rope(T, H, hd, rot, dtype, interleaved):
         assert torch.equal(_bits(y), _bits(got))
 
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_rope_strides(dtype, interleaved):
     """Slices of a joint projection, rows at odd offsets, head-major arrays: the bits of the packed call."""
