@@ -32,14 +32,15 @@
 //         dims each for P V, so a chunk's loads are all in flight at once.
 //   many  128-row tiles, 32 rows a wave; K and V tiles go through LDS, loaded
 //         ahead, and are read by all four waves.
-// fp32 (the framework's exact mode) takes one wave per row, VALU sums.
+// fp32 (the framework's exact mode) is the same with v_mfma_f32_16x16x4_f32, 4 keys or dims
+// at a time, exact products and unrounded weights.
 //
 // Rows that a tile's rows do not all see.  Scores outside [lo, hi) become -inf.
 // Keys outside the union of the tile's ranges, and keys of bad pages, are loaded
 // from a row of zeros instead.  Only keys between can carry a neighbour's
-// infinities or NaN into a row (0 * inf in P V): tiles with such keys
-// zero V's non-finite elements for the product and add them, times their
-// weights, to the rows that do see them.
+// infinities or NaN into a row (0 * inf in P V): in tiles with such keys each wave looks
+// through the V rows it loaded, before the workgroup meets, and zeroes what is not
+// finite; if there was any, the rows that do see it get weight times value afterwards.
 #include <type_traits>
 
 #include "common.h"
@@ -58,7 +59,7 @@ __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__bf16 x) { return (float)x; }
 __device__ __forceinline__ float to_f(_Float16 x) { return (float)x; }
 
-alignas(16) static __device__ const uint32_t kZeroRow[64] = {};  // a K or V row of zeros (head_dim <= 128, 16 bits)
+alignas(16) static __device__ const uint32_t kZeroRow[128] = {};  // a K or V row of zeros (128 fp32 values at most)
 
 struct AttnP {
   const void *q, *k, *v;
@@ -71,7 +72,7 @@ struct AttnP {
   uint32_t kv_page, kv_slot;
   float scale, softcap, scale2;  // scale2 = scale * log2(e)
   int B, W, H, Hkv, G, width, shift, cap, window;
-  FastDiv by_g, by_hkv, by_b, by_tiles;  // by_tiles: row tiles of a segment (cu = NULL)
+  FastDiv by_g, by_hkv, by_b, by_pairs, by_tiles;  // by_tiles: row tiles of a segment (cu = NULL)
   // chunk partials: part[(row * nc + c) * HD + d] and ml[row * nc + c], row = t * H + h
   float* part;
   float2* ml;
@@ -88,38 +89,35 @@ struct RowTile {
 };
 
 // Which tile slot `slot` is, of `br` rows; every wave finds it for itself, 64
-// segments per step.  The first workgroup also checks that cu ascends.
+// segments per step, each lane with one's bounds and position.  The first workgroup
+// also checks that cu ascends (the search itself is safe with any).
 __device__ __forceinline__ RowTile find_tile(const AttnP& a, int slot, int br, int lane, bool first) {
   RowTile t;
-  int c0, c1;
-  if (a.cu) {
-    int b = 0;
-    bool bad = false;
-    for (int i = 0; i < a.B; i += WAVE) {
-      const int j = i + lane < a.B ? i + lane + 1 : a.B;
-      int c = a.cu[j];
-      if (first) bad = bad || c < a.cu[j - 1] || c > a.T;
-      c = c < 0 ? 0 : c > a.T ? (int)a.T : c;
-      b += __builtin_popcountll(__ballot(i + lane < a.B && first_slot(c, a.G, br, j) <= slot));
-    }
-    if (first && __any(bad) && lane == 0) flag_err(a.err, ALTXS_EDEV_POS);
-    t.b = __builtin_amdgcn_readfirstlane(b);
-    if (t.b >= a.B) {
-      t.r0 = t.rows = 0;
-      return t;
-    }
-    c0 = a.cu[t.b];
-    c1 = a.cu[t.b + 1];
-    t.s = segment_of(c0, c1, a.pos[t.b], a.T, a.cap);
-    const int64_t j = slot - first_slot(t.s.t0, a.G, br, t.b);
-    t.rows = t.s.n * a.G;
-    t.r0 = j < 0 || j * br >= t.rows ? t.rows : (int)(j * br);
-  } else {
+  t.b = a.B;
+  t.r0 = t.rows = 0;
+  if (!a.cu) {
     t.b = (int)div_by(slot, a.by_tiles);
-    c0 = t.b * a.W;
+    const int c0 = t.b * a.W;
     t.s = segment_of(c0, c0 + a.W, a.pos[t.b], a.T, a.cap);
     t.rows = a.W * a.G;
     t.r0 = (slot - t.b * (int)a.by_tiles.d) * br;
+    return t;
+  }
+  for (int i = 0; i < a.B; i += WAVE) {
+    const int j = i + lane < a.B ? i + lane : a.B - 1;
+    const int c0 = a.cu[j], c1 = a.cu[j + 1], p = a.pos[j];
+    if (first && __any(c1 < c0 || c1 > a.T || (j == 0 && c0 != 0)) && lane == 0) flag_err(a.err, ALTXS_EDEV_POS);
+    const int e = c1 < 0 ? 0 : c1 > a.T ? (int)a.T : c1;
+    const uint64_t later = __ballot(i + lane < a.B && first_slot(e, a.G, br, j + 1) > slot);
+    if (later && t.b == a.B) {
+      const int n = __builtin_ctzll(later);
+      t.b = i + n;
+      t.s = segment_of(__builtin_amdgcn_readlane(c0, n), __builtin_amdgcn_readlane(c1, n), __builtin_amdgcn_readlane(p, n), a.T, a.cap);
+      const int64_t k = slot - first_slot(t.s.t0, a.G, br, t.b);
+      t.rows = t.s.n * a.G;
+      t.r0 = k < 0 || k * br >= t.rows ? t.rows : (int)(k * br);
+      if (!first) break;
+    }
   }
   return t;
 }
@@ -184,6 +182,30 @@ __device__ __forceinline__ Seen both(const Seen a, const Seen b) {
   return {a.lo < b.lo ? a.lo : b.lo, a.hi > b.hi ? a.hi : b.hi, a.clo > b.clo ? a.clo : b.clo, a.chi < b.chi ? a.chi : b.chi};
 }
 
+// ---- keys ----------------------------------------------------------------------
+
+// The table entry of a key, read for the nearest key of the rows' union [LO, HI)
+// (LO < HI <= what the table holds), and the page it names: -1 for a key outside the
+// union or an entry that is no page (flagged).
+__device__ __forceinline__ int key_entry(const AttnP& a, int b, int key, int LO, int HI) {
+  const int k = key < LO ? LO : key >= HI ? HI - 1 : key;
+  return a.table[(int64_t)b * a.width + (k >> a.shift)];
+}
+__device__ __forceinline__ int entry_page(const AttnP& a, int entry, int key, int LO, int HI) {
+  const bool seen = key >= LO && key < HI, good = entry >= 0 && entry < a.n_pages;
+  if (seen && !good) flag_err(a.err, ALTXS_EDEV_PAGE);
+  return seen && good ? entry : -1;
+}
+
+// A key's row of kv head hk (head = its offset) in a cache, or the row of zeros.
+template <class T>
+__device__ __forceinline__ const T* key_row(const void* cache, int page, int key, int shift, uint32_t st_page, uint32_t st_slot,
+                                            int64_t head) {
+  const int64_t at = (int64_t)((uint64_t)(page < 0 ? 0 : page) * st_page + (uint64_t)(key & ((1 << shift) - 1)) * st_slot) + head;
+  const T* p = (const T*)cache + at;
+  return page < 0 ? (const T*)kZeroRow : p;
+}
+
 // ---- tile arithmetic ---------------------------------------------------------
 
 // The same value, where rare paths start from it: what they compute stays in them
@@ -193,35 +215,38 @@ __device__ __forceinline__ int unhoisted(int x) {
   return x;
 }
 
+// Operands come in 16-byte pieces a lane: EL elements of each of the 4 lane groups, 4 EL
+// along the contraction.  mfma(): the product of two pieces; fp32 has them as four
+// v_mfma_f32_16x16x4_f32, whose k-th slice is element j of lane group k.
 template <class T> struct Op;
 template <> struct Op<__bf16> {
-  typedef bf16x8 vec;
-  static constexpr uint32_t EXP = 0x7f807f80u, ONE = 0x00800080u;  // exponent fields of a pair, their lowest bits
-  static constexpr uint32_t ONES = 0x3f803f80u;                    // a pair of ones
+  static constexpr int EL = 8;
+  static constexpr uint32_t EXP = 0x7f807f80u, ONE = 0x00800080u;  // exponent fields of a word, their lowest bits
+  static constexpr uint32_t TOP = 0x80008000u, ONES = 0x3f803f80u; // the bits above them; a word of ones
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
 };
 template <> struct Op<_Float16> {
-  typedef f16x8 vec;
-  static constexpr uint32_t EXP = 0x7c007c00u, ONE = 0x04000400u, ONES = 0x3c003c00u;
+  static constexpr int EL = 8;
+  static constexpr uint32_t EXP = 0x7c007c00u, ONE = 0x04000400u, TOP = 0x80008000u, ONES = 0x3c003c00u;
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
 };
-
-// The weights of a step's 32 keys (score blocks 2 s, 2 s + 1) as its P operand,
-// rounded to the nearest value of the type.
-template <class T>
-__device__ __forceinline__ u32x4 p_operand(const f32x4 a, const f32x4 b) {
-  typename Op<T>::vec v;
+template <> struct Op<float> {
+  static constexpr int EL = 4;
+  static constexpr uint32_t EXP = 0x7f800000u, ONE = 0x00800000u, TOP = 0x80000000u, ONES = 0x3f800000u;
+  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[i] = (T)a[i];
-    v[4 + i] = (T)b[i];
+    for (int j = 0; j < 4; ++j)
+      c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
+    return c;
   }
-  return __builtin_bit_cast(u32x4, v);
-}
+};
+// Steps of P V over a tile: 32 keys (two score blocks) in the 16-bit types, 16 in fp32.
+template <class T> constexpr int STEPS = TILE / (4 * Op<T>::EL);
+template <class T, int HD> constexpr int PIECES = HD * (int)sizeof(T) / 16;  // of a K or V row
 
 // The larger of two, NaN left out (fmaxf on values out of lane swaps would quiet them first).
 __device__ __forceinline__ float max2(uint32_t a, uint32_t b) {
@@ -291,28 +316,29 @@ __device__ __forceinline__ float next_max(float& m, float mx) {
   return m == old ? 1.f : __builtin_amdgcn_exp2f(old - m);
 }
 
-// Scores -> weights 2^(s - m), as the P operands of the tile's two steps.
+// Scores of step s -> weights 2^(s - m), as its P operand: rounded to the nearest value
+// of a 16-bit type.
 template <class T, bool BIAS>
-__device__ __forceinline__ void tile_weights(const AttnP& a, const f32x4 (&S)[4], float m, u32x4 (&P)[2]) {
+__device__ __forceinline__ u32x4 step_weights(const AttnP& a, const f32x4 (&S)[4], int s, float m) {
 #pragma clang fp contract(off)
   const float mu = m == -INFINITY ? 0.f : m, sc = BIAS ? 1.f : a.scale2;
-  f32x4 w[4];
+  typedef __attribute__((ext_vector_type(Op<T>::EL))) T vec;
+  vec w;
 #pragma unroll
-  for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[kb][i], sc, -mu));
-  P[0] = p_operand<T>(w[0], w[1]);
-  P[1] = p_operand<T>(w[2], w[3]);
+  for (int j = 0; j < Op<T>::EL; ++j)
+    w[j] = (T)__builtin_amdgcn_exp2f(__builtin_fmaf(S[s * Op<T>::EL / 4 + j / 4][j % 4], sc, -mu));
+  return __builtin_bit_cast(u32x4, w);
 }
 
-// V tiles in LDS: rows of HD elements whose 16-byte pieces are permuted so that the
-// 32-byte reads of eight consecutive rows fall into different banks.
-template <int HD> __device__ __forceinline__ int v_piece(int row, int piece) {
-  return piece ^ (HD == 64 ? 2 * ((row >> 1) & 3) : 2 * (row & 7));
+// V tiles in LDS: rows whose 16-byte pieces are permuted so that what a read takes of
+// several rows falls into different banks -- 32 bytes of eight consecutive rows (16-bit
+// types), 64 bytes of every fourth row (fp32).
+template <class T, int HD> __device__ __forceinline__ int v_piece(int row, int piece) {
+  return piece ^ (sizeof(T) == 4 ? 4 * ((row >> 2) & 3) : HD == 64 ? 2 * ((row >> 1) & 3) : 2 * (row & 7));
 }
 // K tiles: a lane reads whole pieces, 16 consecutive rows at the same one.
-template <int HD> __device__ __forceinline__ int k_piece(int row, int piece) {
-  return piece ^ (HD == 64 ? (row >> 1) & 7 : row & 15);
+template <class T, int HD> __device__ __forceinline__ int k_piece(int row, int piece) {
+  return piece ^ (PIECES<T, HD> == 8 ? (row >> 1) & 7 : row & 15);
 }
 
 typedef __attribute__((__vector_size__(4 * sizeof(short)))) short i16x4;
@@ -326,95 +352,107 @@ __device__ __forceinline__ void load_lds16(const void* src, void* dst) {
   __builtin_amdgcn_global_load_lds((glob_void*)src, (lds_void*)dst, 16, 0, 0);
 }
 
-// V operand of step s, dims 16 nb ..: ds_read_b64_tr_b16 gives lane i of each 16
-// lanes element i & 3 of the 8-byte pieces that lanes (i >> 2) + 4 j address, j < 4.
-template <int HD>
-__device__ __forceinline__ u32x4 v_operand(const uint16_t* vt, int s, int nb, int lane) {
+// V operand of step s, dims 16 nb ..  16-bit types: ds_read_b64_tr_b16 gives lane i of each
+// 16 lanes element i & 3 of the 8-byte pieces that lanes (i >> 2) + 4 j address, j < 4.
+template <class T, int HD>
+__device__ __forceinline__ u32x4 v_operand(const T* vt, int s, int nb, int lane) {
   const int g = lane >> 4, col = lane & 15;
-  u32x2 h[2];
+  if constexpr (sizeof(T) == 4) {
+    u32x4 v;
 #pragma unroll
-  for (int jb = 0; jb < 2; ++jb) {
-    const int row = 32 * s + 16 * jb + 4 * g + (col >> 2);
-    const uint16_t* at = vt + row * HD + 8 * v_piece<HD>(row, 2 * nb + ((col & 3) >> 1)) + 4 * (col & 1);
-    h[jb] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)at));
+    for (int j = 0; j < 4; ++j) {
+      const int row = 16 * s + 4 * g + j;
+      v[j] = __float_as_uint(vt[row * HD + 4 * v_piece<T, HD>(row, 4 * nb + (col >> 2)) + (col & 3)]);
+    }
+    return v;
+  } else {
+    u32x2 h[2];
+#pragma unroll
+    for (int jb = 0; jb < 2; ++jb) {
+      const int row = 32 * s + 16 * jb + 4 * g + (col >> 2);
+      const T* at = vt + row * HD + 8 * v_piece<T, HD>(row, 2 * nb + ((col & 3) >> 1)) + 4 * (col & 1);
+      h[jb] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)at));
+    }
+    return u32x4{h[0][0], h[0][1], h[1][0], h[1][1]};
   }
-  return u32x4{h[0][0], h[0][1], h[1][0], h[1][1]};
 }
 
-// O += P V over one tile, dims 16 (nb0 + nb) ..; O[cb][nb]: row block cb.  l += the
-// sum of the weights, a product with ones: every register holds the row's sum (of the
-// rounded weights, so that they add up to one after the division).
-template <class T, int HD, int CB, int NB>
-__device__ __forceinline__ void tile_pv(f32x4 (&O)[CB][NB], f32x4 (&l)[CB], const u32x4 (&P)[CB][2], const uint16_t* vt, int nb0,
-                                        bool mixed, const Row (&r)[CB], int k0, int lane) {
-#pragma clang fp contract(off)
-  constexpr uint32_t ONES = Op<T>::ONES;
-  const u32x4 ones = {ONES, ONES, ONES, ONES};
+// O += P V over one step's keys; O[cb][nb]: row block cb, 16 dims.  l += the sum of the
+// weights, a product with ones: every register holds the row's sum (of the rounded
+// weights, so that they add up to one after the division).
+template <class T, int CB, int NB>
+__device__ __forceinline__ void step_pv(f32x4 (&O)[CB][NB], f32x4 (&l)[CB], const u32x4 (&P)[CB], const u32x4 (&v)[NB]) {
+  const u32x4 ones = {Op<T>::ONES, Op<T>::ONES, Op<T>::ONES, Op<T>::ONES};
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
+  for (int cb = 0; cb < CB; ++cb) {
+    l[cb] = Op<T>::mfma(ones, P[cb], l[cb]);
 #pragma unroll
-    for (int cb = 0; cb < CB; ++cb) l[cb] = Op<T>::mfma(ones, P[cb][s], l[cb]);
-  if (mixed) {  // does V hold infinities or NaN?  Their sums with anything do (and large sums may: no harm)
-    f32x4 z = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) z = Op<T>::mfma(v_operand<HD>(vt, s, nb0 + nb, lane), ones, z);
-    mixed = __any(!(fabsf(z[0]) < INFINITY && fabsf(z[1]) < INFINITY && fabsf(z[2]) < INFINITY && fabsf(z[3]) < INFINITY));
+    for (int nb = 0; nb < NB; ++nb) O[cb][nb] = Op<T>::mfma(v[nb], P[cb], O[cb][nb]);
   }
-  if (!mixed) {
+}
+
+// Zero what is not finite in the 16 bytes at `at` (LDS); whether there was any.
+template <class T>
+__device__ __forceinline__ bool take_odd(T* at) {
+  u32x4 v = *(u32x4*)at;
+  uint32_t any = 0;
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+  for (int i = 0; i < 4; ++i) {  // a full exponent field carries into the bit above it
+    const uint32_t f = ((v[i] & Op<T>::EXP) + Op<T>::ONE) & Op<T>::TOP;
+    any |= f;
+    v[i] &= ~((f << 1) - (f >> (8 * sizeof(T) - 1)));
+  }
+  if (any) *(u32x4*)at = v;
+  return any != 0;
+}
+
+// The values that take_odd() took out of tile k0's V, read again from their pages, times
+// their weights, to the rows that see them; dims 16 (nb0 + nb) ... Rare.
+template <class T, int HD, int CB, int NB>
+__device__ void add_odd(const AttnP& a, int b, int hk, f32x4 (&O)[CB][NB], const u32x4 (&P)[CB][STEPS<T>], int nb0,
+                        const Row (&r)[CB], int k0, int LO, int HI, int lane) {
+#pragma clang fp contract(off)
+  constexpr int PER = 4 / (int)sizeof(T);  // weights of a register
+  lane = unhoisted(lane);
+  const int g = lane >> 4, col = lane & 15;
+  u32x4 w[CB][STEPS<T>];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const u32x4 v = v_operand<HD>(vt, s, nb0 + nb, lane);
+  for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
-        for (int cb = 0; cb < CB; ++cb) O[cb][nb] = Op<T>::mfma(v, P[cb][s], O[cb][nb]);
-      }
-  } else {  // rare: without those elements, which then go to the rows that see them
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        u32x4 v = v_operand<HD>(vt, s, nb0 + nb, lane);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {  // a full exponent field carries into the bit above it
-          const uint32_t f = ((v[i] & Op<T>::EXP) + Op<T>::ONE) & 0x80008000u;
-          v[i] &= ~((f << 1) - (f >> 15));
-        }
-#pragma unroll
-        for (int cb = 0; cb < CB; ++cb) O[cb][nb] = Op<T>::mfma(v, P[cb][s], O[cb][nb]);
-      }
-    lane = unhoisted(lane);
-    const int g = lane >> 4, col = lane & 15;
-#pragma unroll
-    for (int cb = 0; cb < CB; ++cb) {
-      u32x4 w[2] = {P[cb][0], P[cb][1]};
+    for (int s = 0; s < STEPS<T>; ++s) w[cb][s] = P[cb][s];
 #pragma unroll 1
-      for (int n = 0; n < 8; ++n) {  // pair n of a lane's weights: keys 16 (n / 2) + 4 g + 2 (n % 2) + {0, 1}
-        const uint32_t pair = w[0][0];
-        w[0] = u32x4{w[0][1], w[0][2], w[0][3], w[1][0]};
-        w[1] = u32x4{w[1][1], w[1][2], w[1][3], pair};
+  for (int n = 0; n < 16 / PER; ++n) {  // register n of a lane's weights: its keys PER n .. (of 4 a block: 16 (. / 4) + 4 g + . % 4)
+    uint32_t x[CB];
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {  // taken from the front, the others moved up
+      x[cb] = w[cb][0][0];
+#pragma unroll
+      for (int s = 0; s < STEPS<T>; ++s)
+        w[cb][s] = u32x4{w[cb][s][1], w[cb][s][2], w[cb][s][3], s + 1 < STEPS<T> ? w[cb][(s + 1) % STEPS<T>][0] : x[cb]};
+    }
 #pragma unroll 1
-        for (int q = 0; q < 8; ++q) {
-          const int src = q >> 1, half = q & 1;
-          const int row = 16 * (n >> 1) + 4 * src + 2 * (n & 1) + half, key = k0 + row;
-          const uint32_t both = __shfl(pair, 16 * src + col, WAVE);
-          const float p = to_f(__builtin_bit_cast(T, (uint16_t)(half ? both >> 16 : both)));
+    for (int q = 0; q < 4 * PER; ++q) {
+      const int src = q / PER, of = q % PER, j = PER * n + of, key = k0 + 16 * (j >> 2) + 4 * src + (j & 3);
+      if (key < LO || key >= HI) continue;
+      const int entry = key_entry(a, b, key, LO, HI);
+      if (entry < 0 || entry >= a.n_pages) continue;
+      const T* v = key_row<T>(a.v, entry, key, a.shift, a.kv_page, a.kv_slot, hk * a.kv_head);
+      float p[CB];
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            const int d = 16 * (nb0 + nb) + 4 * g;
-            const uint16_t* at = vt + row * HD + 8 * v_piece<HD>(row, d >> 3) + (d & 7);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t x = at[i];
-              const bool odd = (x & Op<T>::EXP & 0xffffu) == (Op<T>::EXP & 0xffffu);
-              if (odd && key >= r[cb].lo && key < r[cb].hi)
-                O[cb][nb][i] = __builtin_fmaf(p, to_f(__builtin_bit_cast(T, (uint16_t)x)), O[cb][nb][i]);
-            }
-          }
-        }
+      for (int cb = 0; cb < CB; ++cb) {
+        const uint32_t y = __shfl(x[cb], 16 * src + col, WAVE);
+        if constexpr (PER == 1) p[cb] = __uint_as_float(y);
+        else p[cb] = to_f(__builtin_bit_cast(T, (uint16_t)(of ? y >> 16 : y)));
       }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = to_f(v[16 * (nb0 + nb) + 4 * g + i]);
+#pragma unroll
+          for (int cb = 0; cb < CB; ++cb)
+            if (!(fabsf(e) < INFINITY) && key >= r[cb].lo && key < r[cb].hi) O[cb][nb][i] = __builtin_fmaf(p[cb], e, O[cb][nb][i]);
+        }
     }
   }
 }
@@ -453,38 +491,18 @@ __device__ __forceinline__ void store_part(const AttnP& a, const Row& r, int c, 
   *(f32x4*)(a.part + ((r.t * a.H + r.h) * a.nc + c) * HD + d) = o;
 }
 
-// The table entry of a key, read for the nearest key of the rows' union [LO, HI)
-// (LO < HI <= what the table holds), and the page it names: -1 for a key outside the
-// union or an entry that is no page (flagged).
-__device__ __forceinline__ int key_entry(const AttnP& a, int b, int key, int LO, int HI) {
-  const int k = key < LO ? LO : key >= HI ? HI - 1 : key;
-  return a.table[(int64_t)b * a.width + (k >> a.shift)];
-}
-__device__ __forceinline__ int entry_page(const AttnP& a, int entry, int key, int LO, int HI) {
-  const bool seen = key >= LO && key < HI, good = entry >= 0 && entry < a.n_pages;
-  if (seen && !good) flag_err(a.err, ALTXS_EDEV_PAGE);
-  return seen && good ? entry : -1;
-}
-
-// A key's row of kv head hk (head = its offset) in a cache, or the row of zeros.
-template <class T>
-__device__ __forceinline__ const T* key_row(const void* cache, int page, int key, int shift, uint32_t st_page, uint32_t st_slot,
-                                            int64_t head) {
-  const int64_t at = (int64_t)((uint64_t)(page < 0 ? 0 : page) * st_page + (uint64_t)(key & ((1 << shift) - 1)) * st_slot) + head;
-  const T* p = (const T*)cache + at;
-  return page < 0 ? (const T*)kZeroRow : p;
-}
-
 // ---- few rows ----------------------------------------------------------------
 
 template <class T, int HD, bool BIAS>
 __global__ __launch_bounds__(THREADS) void attn_few_kernel(AttnP a) {
 #pragma clang fp contract(off)
-  constexpr int KS = HD / 32, NB = HD / 16 / WAVES;      // k-steps of a score; 16-dim blocks of a wave's share of O
-  constexpr int PR = HD / 8, RPL = WAVE / PR;            // 16-byte pieces of a row; rows of one LDS load
-  __shared__ alignas(16) uint16_t vt[TPC][TILE * HD];
-  __shared__ u32x4 pt[TPC][2][WAVE];
+  constexpr int EL = Op<T>::EL, KS = HD / (4 * EL), ST = STEPS<T>;  // pieces of a score; steps of P V
+  constexpr int NB = HD / 16 / WAVES;                              // 16-dim blocks of a wave's share of O
+  constexpr int PR = PIECES<T, HD>, RPL = WAVE / PR;               // rows of one LDS load
+  __shared__ alignas(16) T vt[TPC][TILE * HD];
+  __shared__ u32x4 pt[TPC][ST][WAVE];
   __shared__ float tmax[TPC][16];
+  __shared__ int odd[TPC];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE;
   const int g = lane >> 4, col = lane & 15;
   const int slot = (int)div_by(blockIdx.x, a.by_hkv), hk = blockIdx.x - slot * a.Hkv;
@@ -497,7 +515,7 @@ __global__ __launch_bounds__(THREADS) void attn_few_kernel(AttnP a) {
   u32x4 q[KS];
 #pragma unroll
   for (int s = 0; s < KS; ++s)
-    q[s] = r.valid ? *(const u32x4*)((const T*)a.q + r.t * a.q_tok + r.h * a.q_head + 32 * s + 8 * g) : u32x4{0, 0, 0, 0};
+    q[s] = r.valid ? *(const u32x4*)((const T*)a.q + r.t * a.q_tok + r.h * a.q_head + EL * (4 * s + g)) : u32x4{0, 0, 0, 0};
   float M = -INFINITY, L = 0.f;
   f32x4 O[NB];
 #pragma unroll
@@ -513,13 +531,13 @@ __global__ __launch_bounds__(THREADS) void attn_few_kernel(AttnP a) {
         const int i = 16 * kb + col;
         const T* src = key_row<T>(a.k, __shfl(pg, i, WAVE), k0 + i, a.shift, a.kv_page, a.kv_slot, hk * a.kv_head);
 #pragma unroll
-        for (int s = 0; s < KS; ++s) k[kb][s] = *(const u32x4*)(src + 32 * s + 8 * g);
+        for (int s = 0; s < KS; ++s) k[kb][s] = *(const u32x4*)(src + EL * (4 * s + g));
       }
 #pragma unroll
       for (int i = 0; i < TILE / RPL; ++i) {
         const int vr = i * RPL + lane / PR;
         const T* src = key_row<T>(a.v, __shfl(pg, vr, WAVE), k0 + vr, a.shift, a.kv_page, a.kv_slot, hk * a.kv_head);
-        load_lds16(src + 8 * v_piece<HD>(vr, lane % PR), vt[wave] + i * RPL * HD);
+        load_lds16(src + EL * v_piece<T, HD>(vr, lane % PR), vt[wave] + i * RPL * HD);
       }
       f32x4 S[1][4];
 #pragma unroll
@@ -538,11 +556,16 @@ __global__ __launch_bounds__(THREADS) void attn_few_kernel(AttnP a) {
         al[t] = next_max(m, tmax[t][col]);
         if (t == wave) mw = m;
       }
-      u32x4 w[2];
-      tile_weights<T, BIAS>(a, S[0], mw, w);
-      pt[wave][0][lane] = w[0];
-      pt[wave][1][lane] = w[1];
-      __builtin_amdgcn_s_waitcnt(0);  // the V tiles
+#pragma unroll
+      for (int s = 0; s < ST; ++s) pt[wave][s][lane] = step_weights<T, BIAS>(a, S[0], s, mw);
+      __builtin_amdgcn_s_waitcnt(0);  // the wave's V tile
+      if (seen.mixed(k0, seen.lo, seen.hi)) {
+        bool found = false;
+#pragma unroll
+        for (int i = 0; i < TILE / RPL; ++i) found |= take_odd<T>(vt[wave] + i * RPL * HD + EL * lane);
+        const bool any = __any(found);
+        if (lane == 0) odd[wave] = any;
+      }
       __syncthreads();
       f32x4 l[1] = {f32x4{0.f, 0.f, 0.f, 0.f}}, o[1][NB];
 #pragma unroll
@@ -552,9 +575,19 @@ __global__ __launch_bounds__(THREADS) void attn_few_kernel(AttnP a) {
         l[0] *= al[t];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) o[0][nb] *= al[t];
-        const u32x4 P[1][2] = {{pt[t][0][lane], pt[t][1][lane]}};
+        u32x4 P[1][ST];
+#pragma unroll
+        for (int s = 0; s < ST; ++s) {
+          u32x4 v[NB];
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) v[nb] = v_operand<T, HD>(vt[t], s, wave * NB + nb, lane);
+          P[0][s] = pt[t][s][lane];
+          const u32x4 Ps[1] = {P[0][s]};
+          step_pv<T, 1, NB>(o, l, Ps, v);
+        }
         const int kt = c * CHUNK + t * TILE;
-        tile_pv<T, HD, 1, NB>(o, l, P, vt[t], wave * NB, seen.mixed(kt, seen.lo, seen.hi), row, kt, lane);
+        if (seen.mixed(kt, seen.lo, seen.hi) && odd[t])
+          add_odd<T, HD, 1, NB>(a, tile.b, hk, o, P, wave * NB, row, kt, seen.lo, seen.hi, lane);
       }
       if (a.direct) {
         const Fold f = fold(M, L, m, l[0][0]);
@@ -581,30 +614,41 @@ __global__ __launch_bounds__(THREADS) void attn_few_kernel(AttnP a) {
 
 constexpr int NW = 4;  // waves of a workgroup
 // 16-row blocks of a wave, and rows of a workgroup
-template <int HD> constexpr int many_cb = HD == 64 ? 2 : 1;
-template <int HD> constexpr int many_rows = NW * 16 * many_cb<HD>;
+template <class T, int HD> constexpr int many_cb = HD * sizeof(T) == 128 ? 2 : 1;
+template <class T, int HD> constexpr int many_rows = NW * 16 * many_cb<T, HD>;
 
-// The last row tiles of a segment see the most keys: they go first -- of equal segments
-// all last tiles, then all second to last ones; of ragged ones the slots backwards.
-__device__ __forceinline__ int many_slot(const AttnP& a, int i) {
-  if (a.cu) return (int)(gridDim.x / a.Hkv) - 1 - i;
-  const int back = (int)div_by(i, a.by_b), b = i - back * a.B;
-  return (b + 1) * (int)a.by_tiles.d - 1 - back;
+// Workgroup i -> (slot, kv head).  The last row tiles of a segment see the most keys:
+// they go first -- of equal segments all last tiles, then all second to last ones, each
+// over (kv head, segment) with the segment running fastest: workgroups are dealt to the
+// 8 XCDs in turn, so (for a multiple of 8 pairs) a pair's tiles share an L2, and an XCD's
+// pairs spread over it (all of one kv head they would meet in an eighth of its sets:
+// pages of 64 KB hold 8 KB a head).  Ragged segments: the slots backwards.
+__device__ __forceinline__ int many_slot(const AttnP& a, int i, int& hk) {
+  if (a.cu) {
+    const int slot = (int)div_by(i, a.by_hkv);
+    hk = i - slot * a.Hkv;
+    return (int)(gridDim.x / a.Hkv) - 1 - slot;
+  }
+  const int back = (int)div_by(i, a.by_pairs), pair = i - back * (int)a.by_pairs.d;
+  hk = (int)div_by(pair, a.by_b);
+  return (pair - hk * a.B + 1) * (int)a.by_tiles.d - 1 - back;
 }
 
 template <class T, int HD, bool BIAS>
 __global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
 #pragma clang fp contract(off)
-  constexpr int CB = many_cb<HD>, MANY = many_rows<HD>, KS = HD / 32, NB = HD / 16;
-  constexpr int PR = HD / 8, RPW = WAVE / PR, RPL = NW * RPW, LOADS = TILE / RPL;  // rows of a wave's load, of the workgroup's; loads
-  static_assert(RPL % 16 == 0 && RPW <= 16, "a load's rows lie in one page, its pieces are permuted alike");
+  constexpr int CB = many_cb<T, HD>, MANY = many_rows<T, HD>, EL = Op<T>::EL, KS = HD / (4 * EL), ST = STEPS<T>, NB = HD / 16;
+  constexpr int PR = PIECES<T, HD>, RPW = WAVE / PR, RPL = NW * RPW, LOADS = TILE / RPL;  // rows of a wave's load, of the workgroup's; loads
+  static_assert(16 % RPW == 0 && RPL % 8 == 0, "a load's rows lie in one page");
+  constexpr int KINDS = RPL % 16 == 0 ? 1 : 2;  // pieces are permuted by the row modulo 16: alike in every load, or in every other
   // separate arrays: reads of one buffer do not wait for the loads into the other
-  __shared__ alignas(16) uint16_t kt0[TILE * HD], kt1[TILE * HD], vt0[TILE * HD], vt1[TILE * HD];
-  __shared__ int range[4][NW];
+  __shared__ alignas(16) T kt0[TILE * HD], kt1[TILE * HD], vt0[TILE * HD], vt1[TILE * HD];
+  __shared__ int range[4][NW], odd[2][NW];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE;
   const int g = lane >> 4, col = lane & 15;
-  const int slot = (int)div_by(blockIdx.x, a.by_hkv), hk = blockIdx.x - slot * a.Hkv;
-  const RowTile tile = find_tile(a, many_slot(a, slot), MANY, lane, blockIdx.x == 0 && blockIdx.y == 0 && wave == 0);
+  int hk;
+  const int slot = many_slot(a, blockIdx.x, hk);
+  const RowTile tile = find_tile(a, slot, MANY, lane, blockIdx.x == 0 && blockIdx.y == 0 && wave == 0);
   if (tile.r0 >= tile.rows) return;
   if (!tile.s.ok && threadIdx.x == 0) flag_err(a.err, ALTXS_EDEV_POS);
   Row r[CB];
@@ -614,7 +658,7 @@ __global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
     r[cb] = row_of(a, tile, hk, tile.r0 + 16 * (wave * CB + cb) + col);
 #pragma unroll
     for (int s = 0; s < KS; ++s)
-      q[cb][s] = r[cb].valid ? *(const u32x4*)((const T*)a.q + r[cb].t * a.q_tok + r[cb].h * a.q_head + 32 * s + 8 * g)
+      q[cb][s] = r[cb].valid ? *(const u32x4*)((const T*)a.q + r[cb].t * a.q_tok + r[cb].h * a.q_head + EL * (4 * s + g))
                              : u32x4{0, 0, 0, 0};
   }
   Seen seen = seen_by(r[0]);
@@ -632,8 +676,9 @@ __global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
   for (int w = 0; w < NW; ++w) all = both(all, Seen{range[0][w], range[1][w], range[2][w], range[3][w]});
   const int LO = __builtin_amdgcn_readfirstlane(all.lo), HI = __builtin_amdgcn_readfirstlane(all.hi);
   // tiles [in0, in1) are seen whole by every row of the workgroup
-  const int in0 = (__builtin_amdgcn_readfirstlane(all.clo) + TILE - 1) / TILE;
-  const int in1 = __builtin_amdgcn_readfirstlane(all.chi) / TILE;
+  all.clo = __builtin_amdgcn_readfirstlane(all.clo);
+  all.chi = __builtin_amdgcn_readfirstlane(all.chi);
+  const int in0 = (all.clo + TILE - 1) / TILE, in1 = all.chi / TILE;
 
   float m[CB], M[CB], L[CB];
   f32x4 l[CB], O[CB][NB], Ot[CB][NB];
@@ -648,7 +693,7 @@ __global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
 
   const int t_end = LO < HI ? (HI + TILE - 1) / TILE : 0, skip = TPC * ((int)gridDim.y - 1);
   auto after = [&](int t) { return (t & (TPC - 1)) == TPC - 1 ? t + 1 + skip : t + 1; };
-  // Loads go by whole waves, 8 (4) rows at a time, all in one page, whose entry is a
+  // Loads go by whole waves, 2 to 8 rows at a time, all in one page, whose entry is a
   // scalar; with pages of a tile or more one entry serves the whole tile.  Entries are
   // read for the nearest tile or key of the union (inside the table).
   const const_i32* entries = (const const_i32*)(a.table + (int64_t)tile.b * a.width);
@@ -671,18 +716,22 @@ __global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
   const int whole0 = (LO + TILE - 1) / TILE;  // tiles all of whose keys are in the union
   const uint32_t wholes = HI / TILE > whole0 ? HI / TILE - whole0 : 0;
   const int krow = wave * RPW + lane / PR;
-  const T* kl = (const T*)a.k + hk * a.kv_head + (uint64_t)krow * a.kv_slot + 8 * k_piece<HD>(krow, lane % PR);
-  const T* vl = (const T*)a.v + hk * a.kv_head + (uint64_t)krow * a.kv_slot + 8 * v_piece<HD>(krow, lane % PR);
+  const T *kl[KINDS], *vl[KINDS];
+#pragma unroll
+  for (int i = 0; i < KINDS; ++i) {
+    kl[i] = (const T*)a.k + hk * a.kv_head + (uint64_t)krow * a.kv_slot + EL * k_piece<T, HD>(krow + i * RPL, lane % PR);
+    vl[i] = (const T*)a.v + hk * a.kv_head + (uint64_t)krow * a.kv_slot + EL * v_piece<T, HD>(krow + i * RPL, lane % PR);
+  }
   const uint64_t down = RPL * (uint64_t)a.kv_slot;  // a load's rows to the next one's
-  auto load = [&](int t, const int (&e)[LOADS], uint16_t* kb, uint16_t* vb) {
+  auto load = [&](int t, const int (&e)[LOADS], T* kb, T* vb) {
     const bool whole = (uint32_t)(t - whole0) < wholes;
     if (large && whole && (uint32_t)e[0] < n_pages) {
       uint64_t at = (uint64_t)(uint32_t)e[0] * a.kv_page + (uint64_t)(uint32_t)((t << 6) & ((1 << a.shift) - 1)) * a.kv_slot;
 #pragma unroll
       for (int i = 0; i < LOADS; ++i, at += down) {
         const int to = (i * RPL + wave * RPW) * HD;
-        load_lds16(kl + at, kb + to);
-        load_lds16(vl + at, vb + to);
+        load_lds16(kl[i % KINDS] + at, kb + to);
+        load_lds16(vl[i % KINDS] + at, vb + to);
       }
       return;
     }
@@ -693,16 +742,16 @@ __global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
       // kl and vl already stand krow rows into the page
       const uint64_t at = (uint64_t)(good ? (uint32_t)entry : 0) * a.kv_page +
                           (int64_t)((key & ((1 << a.shift) - 1)) - wave * RPW) * (int64_t)a.kv_slot;
-      const T* ks = kl + at;
-      const T* vs = vl + at;
+      const T* ks = kl[i % KINDS] + at;
+      const T* vs = vl[i % KINDS] + at;
       const int to = (first + wave * RPW) * HD;
       if (!(whole && good)) {
-        const int ln = unhoisted(lane), row = wave * RPW + ln / PR;
+        const int ln = unhoisted(lane), row = first + wave * RPW + ln / PR;
         const bool in = key + ln / PR >= LO && key + ln / PR < HI;
         if (in && !good) flag_err(a.err, ALTXS_EDEV_PAGE);
         if (!in || !good) {
-          ks = (const T*)kZeroRow + 8 * k_piece<HD>(row, ln % PR);
-          vs = (const T*)kZeroRow + 8 * v_piece<HD>(row, ln % PR);
+          ks = (const T*)kZeroRow + EL * k_piece<T, HD>(row, ln % PR);
+          vs = (const T*)kZeroRow + EL * v_piece<T, HD>(row, ln % PR);
         }
       }
       load_lds16(ks, kb + to);
@@ -711,8 +760,8 @@ __global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
   };
 
   int t = 0, tn = 0;
-  // One tile out of (kb, vb).  EDGE: some row does not see it whole.
-  auto work = [&](auto edge, const uint16_t* kb, const uint16_t* vb) {
+  // One tile out of (kb, vb), buffer buf.  EDGE: some row does not see it whole.
+  auto work = [&](auto edge, const T* kb, const T* vb, int buf) {
     constexpr bool EDGE = decltype(edge)::value;
     const int k0 = t * TILE;
     if (EDGE && !(seen.lo < k0 + TILE && seen.hi > k0)) return;  // no row of the wave sees any of it
@@ -724,13 +773,12 @@ __global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const int row = 16 * j + col;
-        const u32x4 k = *(const u32x4*)(kb + row * HD + 8 * k_piece<HD>(row, 4 * s + g));
+        const u32x4 k = *(const u32x4*)(kb + row * HD + EL * k_piece<T, HD>(row, 4 * s + g));
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) S[cb][j] = Op<T>::mfma(k, q[cb][s], S[cb][j]);
       }
     }
     float mx[CB], al[CB];
-    u32x4 P[CB][2];
     tile_scores<BIAS, CB>(a, S, mx, r, k0, g, !EDGE || seen.full(k0));
     bool moved = false;
 #pragma unroll
@@ -746,9 +794,35 @@ __global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
         for (int nb = 0; nb < NB; ++nb) O[cb][nb] *= al[cb];
       }
     }
+    u32x4 P[CB][ST];
 #pragma unroll
-    for (int cb = 0; cb < CB; ++cb) tile_weights<T, BIAS>(a, S[cb], m[cb], P[cb]);
-    tile_pv<T, HD, CB, NB>(O, l, P, vb, 0, EDGE && seen.mixed(k0, LO, HI), r, k0, lane);
+    for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+      for (int s = 0; s < ST; ++s) P[cb][s] = step_weights<T, BIAS>(a, S[cb], s, m[cb]);
+#pragma unroll
+    for (int s = 0; s < ST; ++s) {
+      u32x4 v[NB], Ps[CB];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) v[nb] = v_operand<T, HD>(vb, s, nb, lane);
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) Ps[cb] = P[cb][s];
+      step_pv<T, CB, NB>(O, l, Ps, v);
+    }
+    if (EDGE && all.mixed(k0, LO, HI)) {
+      int found = 0;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) found |= odd[buf][w];
+      if (__builtin_amdgcn_readfirstlane(found)) add_odd<T, HD, CB, NB>(a, tile.b, hk, O, P, 0, r, k0, LO, HI, lane);
+    }
+  };
+  // Before the workgroup meets over tile t in buffer buf: the rows that this wave loaded.
+  auto clean = [&](int t, T* vb, int buf) {
+    if (!all.mixed(t * TILE, LO, HI)) return;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) found |= take_odd<T>(vb + (i * RPL + wave * RPW) * HD + EL * lane);
+    const bool any = __any(found);
+    if (lane == 0) odd[buf][wave] = any;
   };
   auto end_chunk = [&]() {
 #pragma unroll
@@ -775,16 +849,17 @@ __global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
   // (kn, vn), and the entries of the one after it are read; false after the last.
   int en[LOADS];
   const uint32_t n_in = in1 > in0 ? in1 - in0 : 0;
-  auto step = [&](const uint16_t* kb, const uint16_t* vb, uint16_t* kn, uint16_t* vn) {
+  auto step = [&](const T* kb, const T* vb, T* kn, T* vn, int buf) {
     if (tn < t_end) load(tn, en, kn, vn);
     const int tnn = after(tn);
     lookup(tnn, en);
-    if ((uint32_t)(t - in0) < n_in) work(std::false_type{}, kb, vb);
-    else work(std::true_type{}, kb, vb);
+    if ((uint32_t)(t - in0) < n_in) work(std::false_type{}, kb, vb, buf);
+    else work(std::true_type{}, kb, vb, buf);
     if ((t & (TPC - 1)) == TPC - 1 || tn >= t_end) end_chunk();
     if (tn >= t_end) return false;
-    __builtin_amdgcn_s_waitcnt(0);  // the next tile is there,
-    __syncthreads();                // and this one's buffer free
+    __builtin_amdgcn_s_waitcnt(0);  // the wave's part of the next tile is there
+    clean(tn, vn, buf ^ 1);
+    __syncthreads();  // all of it is, and this one's buffer is free
     t = tn;
     tn = tnn;
     return true;
@@ -796,8 +871,9 @@ __global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
     tn = after(t);
     lookup(tn, en);
     __builtin_amdgcn_s_waitcnt(0);
+    clean(t, vt0, 0);
     __syncthreads();
-    while (step(kt0, vt0, kt1, vt1) && step(kt1, vt1, kt0, vt0)) {}
+    while (step(kt0, vt0, kt1, vt1, 0) && step(kt1, vt1, kt0, vt0, 1)) {}
   }
   if (a.direct) {
 #pragma unroll
@@ -879,91 +955,17 @@ __global__ __launch_bounds__(THREADS) void attn_fold_kernel(AttnP a) {
   for (int i = 0; i < ND; ++i) out[i] = (T)(r.lo < r.hi ? O[i] * inv : 0.f);
 }
 
-// ---- fp32 ----------------------------------------------------------------------
-
-// Scores in the base-2 domain of the softmax: log2(e) (cap tanh(scale x / cap) - slope |p - key|).
-__device__ __forceinline__ float biased(const AttnP& a, float x, float slope, int p, int key) {
-#pragma clang fp contract(off)
-  x *= a.scale;
-  if (a.softcap > 0.f) {
-    const float e = __builtin_amdgcn_exp2f(x * (2.f * LOG2E / a.softcap));
-    x = a.softcap * (1.f - 2.f / (1.f + e));
-  }
-  x *= LOG2E;
-  return __builtin_fmaf(-slope * LOG2E, fabsf((float)(p - key)), x);
-}
-
-// One wave per (token, head): a key per lane for the scores, a dim (or two) per lane
-// for the sum over V.
-template <class T, int HD>
-__global__ __launch_bounds__(THREADS) void attn_row_kernel(AttnP a) {
-#pragma clang fp contract(off)
-  constexpr int ND = HD / WAVE;
-  __shared__ float qs[WAVES][HD];
-  __shared__ float ps[WAVES][TILE];
-  __shared__ int pg[WAVES][TILE];
-  const int wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE;
-  const int64_t row = (int64_t)blockIdx.x * WAVES + wave;
-  if (row >= a.T * a.H) return;
-  const int64_t t = row / a.H;
-  const int h = (int)(row - t * a.H), hk = h / a.G;
-  Segment s;
-  const int b = token_segment(a.cu, a.pos, a.B, a.W, t, a.T, a.cap, lane, s);
-  if (b < 0) return;  // behind the last segment
-  Range r = {0, 0};
-  const int p = s.pos + (int)(t - s.t0);
-  if (s.ok && t >= s.t0)
-    r = keys_seen(p, s.pos + s.n, a.window, a.starts ? a.starts[t] : 0, a.prefix ? a.prefix[b] : 0);
-  else if (lane == 0) flag_err(a.err, ALTXS_EDEV_POS);
-  const T* q = (const T*)a.q + t * a.q_tok + h * a.q_head;
-#pragma unroll
-  for (int i = 0; i < ND; ++i) qs[wave][lane + i * WAVE] = to_f(q[lane + i * WAVE]);
-  const float slope = a.slopes ? a.slopes[h] : 0.f;
-  float m = -INFINITY, l = 0.f, o[ND] = {};
-  for (int k0 = r.lo & ~(TILE - 1); k0 < r.hi; k0 += TILE) {
-    const int key = k0 + lane;
-    int g = -1;
-    float x = -INFINITY;
-    if (key >= r.lo && key < r.hi) {
-      g = page_of(a.table + (int64_t)b * a.width, a.width, a.shift, a.n_pages, key);
-      float acc = 0.f;
-      if (g >= 0) {
-        const T* k = key_row<T>(a.k, g, key, a.shift, a.kv_page, a.kv_slot, hk * a.kv_head);
-#pragma unroll 8
-        for (int d = 0; d < HD; ++d) acc = __builtin_fmaf(qs[wave][d], to_f(k[d]), acc);
-      } else {
-        flag_err(a.err, ALTXS_EDEV_PAGE);
-      }
-      x = biased(a, acc, slope, p, key);
-    }
-    const float mn = fmaxf(m, wave_max(x)), mu = mn == -INFINITY ? 0.f : mn;
-    const float pr = __builtin_amdgcn_exp2f(x - mu), al = __builtin_amdgcn_exp2f(m - mu);
-    ps[wave][lane] = pr;
-    pg[wave][lane] = g;
-    __builtin_amdgcn_wave_barrier();
-    l = __builtin_fmaf(l, al, wave_sum(pr));
-#pragma unroll
-    for (int i = 0; i < ND; ++i) o[i] *= al;
-    for (int j = 0; j < TILE; ++j) {
-      const int gj = pg[wave][j];
-      if (gj < 0) continue;
-      const T* v = key_row<T>(a.v, gj, k0 + j, a.shift, a.kv_page, a.kv_slot, hk * a.kv_head);
-#pragma unroll
-      for (int i = 0; i < ND; ++i) o[i] = __builtin_fmaf(ps[wave][j], to_f(v[lane + i * WAVE]), o[i]);
-    }
-    __builtin_amdgcn_wave_barrier();
-    m = mn;
-  }
-  T* out = (T*)a.out + t * a.o_tok + h * a.o_head;
-#pragma unroll
-  for (int i = 0; i < ND; ++i) out[lane + i * WAVE] = (T)(r.lo < r.hi ? o[i] / l : 0.f);
-}
-
 // ---- host ------------------------------------------------------------------------
 
 // How a call is launched (host decisions only; none of them changes a row's bits).
+// Rows of a tile of the many-row kernel.
+int many(const AltxsPagedAttnArgs* a) {
+  if (a->dtype == ALTXS_F32) return a->head_dim == 64 ? many_rows<float, 64> : many_rows<float, 128>;
+  return a->head_dim == 64 ? many_rows<__bf16, 64> : many_rows<__bf16, 128>;
+}
+
 struct Plan {
-  bool fp32, few;
+  bool few;
   int nc;       // chunks of max_len
   int64_t wgs;  // row-tile slots x kv heads
   int split;    // workgroups that share a row tile's chunks
@@ -972,15 +974,14 @@ struct Plan {
 
 Plan plan_of(const AltxsPagedAttnArgs* a) {
   Plan p = {};
-  p.fp32 = a->dtype == ALTXS_F32;
   p.rows = a->T * a->H;
   p.nc = (a->max_len + CHUNK - 1) / CHUNK;
   if (p.nc < 1) p.nc = 1;
   p.split = 1;
-  if (p.fp32 || a->T == 0 || a->B == 0) return p;
+  if (a->T == 0 || a->B == 0) return p;
   const int G = a->H / a->Hkv;
   p.few = a->T * G <= 16 * (int64_t)a->B;
-  const int br = p.few ? 16 : a->head_dim == 64 ? many_rows<64> : many_rows<128>;
+  const int br = p.few ? 16 : many(a);
   const int64_t slots = a->cu ? slot_count(a->T, G, br, a->B) : (int64_t)a->B * ((a->T / a->B * G + br - 1) / br);
   p.wgs = slots * a->Hkv;
   const int64_t fill = p.few ? 2048 : 512, enough = 384;
@@ -1028,12 +1029,10 @@ extern "C" int32_t altxs_paged_attn(const AltxsPagedAttnArgs* a, altxs_stream_t 
   if (a->T == 0 || a->B == 0) return ALTXS_OK;
   ALTXS_REQUIRE(a->q && a->out && a->k_cache && a->v_cache && a->table && a->pos, "altxs_paged_attn: null pointer");
   const Plan pl = plan_of(a);
-  if (!pl.fp32) {
-    uintptr_t bits = (uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)a->k_cache | (uintptr_t)a->v_cache;
-    for (int64_t st : {a->q_tok, a->q_head, a->out_tok, a->out_head, a->kv_page, a->kv_head, a->kv_slot})
-      bits |= (uintptr_t)(st * 2);
-    ALTXS_REQUIRE((bits & 15) == 0, "altxs_paged_attn: rows of q, out and the caches must start at multiples of 16 bytes");
-  }
+  uintptr_t bits = (uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)a->k_cache | (uintptr_t)a->v_cache;
+  for (int64_t st : {a->q_tok, a->q_head, a->out_tok, a->out_head, a->kv_page, a->kv_head, a->kv_slot})
+    bits |= (uintptr_t)(st * (a->dtype == ALTXS_F32 ? 4 : 2));
+  ALTXS_REQUIRE((bits & 15) == 0, "altxs_paged_attn: rows of q, out and the caches must start at multiples of 16 bytes");
   const int64_t need = ws_bytes(pl, a->head_dim);
   ALTXS_REQUIRE(need == 0 || (a->ws && a->ws_bytes >= need && ((uintptr_t)a->ws & 15) == 0),
                 "altxs_paged_attn: %lld workspace bytes needed, 16-byte aligned (%lld given)", (long long)need,
@@ -1047,8 +1046,8 @@ extern "C" int32_t altxs_paged_attn(const AltxsPagedAttnArgs* a, altxs_stream_t 
   p.scale = a->scale; p.softcap = a->softcap; p.scale2 = a->scale * LOG2E;
   p.B = a->B; p.W = a->cu ? 1 : (int)(a->T / a->B); p.H = a->H; p.Hkv = a->Hkv; p.G = a->H / a->Hkv;
   p.width = a->table_width; p.shift = __builtin_ctz((unsigned)a->page_size); p.cap = a->max_len; p.window = a->window;
-  p.by_g = fast_div(p.G); p.by_hkv = fast_div(p.Hkv); p.by_b = fast_div(p.B);
-  const int br = pl.few ? 16 : a->head_dim == 64 ? many_rows<64> : many_rows<128>;
+  p.by_g = fast_div(p.G); p.by_hkv = fast_div(p.Hkv); p.by_b = fast_div(p.B); p.by_pairs = fast_div((uint32_t)((int64_t)p.B * p.Hkv));
+  const int br = pl.few ? 16 : many(a);
   p.by_tiles = fast_div((uint32_t)(((int64_t)p.W * p.G + br - 1) / br));
   p.nc = pl.nc; p.direct = pl.split == 1;
   p.ml = (float2*)a->ws;  // then O, from a multiple of 16 bytes on
@@ -1061,13 +1060,6 @@ extern "C" int32_t altxs_paged_attn(const AltxsPagedAttnArgs* a, altxs_stream_t 
     if (a->head_dim == 64) hipLaunchKernelGGL((K<T, 64, ##__VA_ARGS__>), grid, block, 0, s, p);  \
     else hipLaunchKernelGGL((K<T, 128, ##__VA_ARGS__>), grid, block, 0, s, p);       \
   } while (0)
-  if (pl.fp32) {
-    using T = float;
-    const dim3 grid = by_row;
-    ALTXS_HD_GO(attn_row_kernel);
-    ALTXS_CHECK_HIP(hipGetLastError());
-    return ALTXS_OK;
-  }
   ALTXS_REQUIRE(pl.wgs < (1ll << 31), "altxs_paged_attn: too many row tiles");
   auto go = [&](auto t) {
     using T = decltype(t);
@@ -1084,7 +1076,8 @@ extern "C" int32_t altxs_paged_attn(const AltxsPagedAttnArgs* a, altxs_stream_t 
       ALTXS_HD_GO(attn_fold_kernel);
     }
   };
-  if (a->dtype == ALTXS_BF16) go(__bf16{});
+  if (a->dtype == ALTXS_F32) go(float{});
+  else if (a->dtype == ALTXS_BF16) go(__bf16{});
   else go(_Float16{});
 #undef ALTXS_HD_GO
   ALTXS_CHECK_HIP(hipGetLastError());

@@ -118,7 +118,7 @@ def test_rows_behind_the_last_segment_and_idle_segments():
     assert (out == 9).all()
 
 
-@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
 @pytest.mark.parametrize("hd", [64, 128])
 def test_bits_do_not_depend_on_the_call(dtype, hd):
     """A row decoded alone, in a batch, in a window, in a whole chunk, on other pages, with a looser bound: the same bits."""
