@@ -40,7 +40,7 @@
 // from a row of zeros instead.  Only keys between can carry a neighbour's
 // infinities or NaN into a row (0 * inf in P V): in tiles with such keys each wave looks
 // through the V rows it loaded, before the workgroup meets, and zeroes what is not
-// finite; if there was any, the rows that do see it get weight times value afterwards.
+// finite; if there was any, it is added to the rows that do see it when the chunk ends.
 #include <type_traits>
 
 #include "common.h"
@@ -406,54 +406,27 @@ __device__ __forceinline__ bool take_odd(T* at) {
   return any != 0;
 }
 
-// The values that take_odd() took out of tile k0's V, read again from their pages, times
-// their weights, to the rows that see them; dims 16 (nb0 + nb) ... Rare.
+// What take_odd() took out of tile k0's V, read again from the pages and added to the
+// rows that see it (weight 1: infinities and NaN, whatever the weight); dims 16 (nb0 + nb)
+// ..  Rare, and kept small so that it costs the loop around it no registers.
 template <class T, int HD, int CB, int NB>
-__device__ void add_odd(const AttnP& a, int b, int hk, f32x4 (&O)[CB][NB], const u32x4 (&P)[CB][STEPS<T>], int nb0,
-                        const Row (&r)[CB], int k0, int LO, int HI, int lane) {
-#pragma clang fp contract(off)
-  constexpr int PER = 4 / (int)sizeof(T);  // weights of a register
-  lane = unhoisted(lane);
-  const int g = lane >> 4, col = lane & 15;
-  u32x4 w[CB][STEPS<T>];
-#pragma unroll
-  for (int cb = 0; cb < CB; ++cb)
-#pragma unroll
-    for (int s = 0; s < STEPS<T>; ++s) w[cb][s] = P[cb][s];
+__device__ __forceinline__ void add_odd(const AttnP& a, int b, int hk, f32x4 (&O)[CB][NB], int nb0, const Row (&r)[CB], int k0,
+                                        int LO, int HI, int lane) {
+  const int first = k0 > LO ? k0 : LO, end = k0 + TILE < HI ? k0 + TILE : HI;
 #pragma unroll 1
-  for (int n = 0; n < 16 / PER; ++n) {  // register n of a lane's weights: its keys PER n .. (of 4 a block: 16 (. / 4) + 4 g + . % 4)
-    uint32_t x[CB];
+  for (int key = first; key < end; ++key) {
+    const int entry = key_entry(a, b, key, LO, HI);
+    if (entry < 0 || entry >= a.n_pages) continue;
+    const T* v = key_row<T>(a.v, entry, key, a.shift, a.kv_page, a.kv_slot, hk * a.kv_head) + 16 * nb0 + 4 * (unhoisted(lane) >> 4);
 #pragma unroll
-    for (int cb = 0; cb < CB; ++cb) {  // taken from the front, the others moved up
-      x[cb] = w[cb][0][0];
+    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int s = 0; s < STEPS<T>; ++s)
-        w[cb][s] = u32x4{w[cb][s][1], w[cb][s][2], w[cb][s][3], s + 1 < STEPS<T> ? w[cb][(s + 1) % STEPS<T>][0] : x[cb]};
-    }
-#pragma unroll 1
-    for (int q = 0; q < 4 * PER; ++q) {
-      const int src = q / PER, of = q % PER, j = PER * n + of, key = k0 + 16 * (j >> 2) + 4 * src + (j & 3);
-      if (key < LO || key >= HI) continue;
-      const int entry = key_entry(a, b, key, LO, HI);
-      if (entry < 0 || entry >= a.n_pages) continue;
-      const T* v = key_row<T>(a.v, entry, key, a.shift, a.kv_page, a.kv_slot, hk * a.kv_head);
-      float p[CB];
+      for (int i = 0; i < 4; ++i) {
+        const float e = to_f(v[16 * nb + i]);
 #pragma unroll
-      for (int cb = 0; cb < CB; ++cb) {
-        const uint32_t y = __shfl(x[cb], 16 * src + col, WAVE);
-        if constexpr (PER == 1) p[cb] = __uint_as_float(y);
-        else p[cb] = to_f(__builtin_bit_cast(T, (uint16_t)(of ? y >> 16 : y)));
+        for (int cb = 0; cb < CB; ++cb)
+          if (!(fabsf(e) < INFINITY) && key >= r[cb].lo && key < r[cb].hi) O[cb][nb][i] += e;
       }
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float e = to_f(v[16 * (nb0 + nb) + 4 * g + i]);
-#pragma unroll
-          for (int cb = 0; cb < CB; ++cb)
-            if (!(fabsf(e) < INFINITY) && key >= r[cb].lo && key < r[cb].hi) O[cb][nb][i] = __builtin_fmaf(p[cb], e, O[cb][nb][i]);
-        }
-    }
   }
 }
 
@@ -575,19 +548,20 @@ __global__ __launch_bounds__(THREADS) void attn_few_kernel(AttnP a) {
         l[0] *= al[t];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) o[0][nb] *= al[t];
-        u32x4 P[1][ST];
 #pragma unroll
         for (int s = 0; s < ST; ++s) {
           u32x4 v[NB];
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) v[nb] = v_operand<T, HD>(vt[t], s, wave * NB + nb, lane);
-          P[0][s] = pt[t][s][lane];
-          const u32x4 Ps[1] = {P[0][s]};
-          step_pv<T, 1, NB>(o, l, Ps, v);
+          const u32x4 P[1] = {pt[t][s][lane]};
+          step_pv<T, 1, NB>(o, l, P, v);
         }
+      }
+#pragma unroll 1
+      for (int t = 0; t < TPC; ++t) {
         const int kt = c * CHUNK + t * TILE;
-        if (seen.mixed(kt, seen.lo, seen.hi) && odd[t])
-          add_odd<T, HD, 1, NB>(a, tile.b, hk, o, P, wave * NB, row, kt, seen.lo, seen.hi, lane);
+        if (seen.mixed(kt, seen.lo, seen.hi) && __builtin_amdgcn_readfirstlane(odd[t]))
+          add_odd<T, HD, 1, NB>(a, tile.b, hk, o, wave * NB, row, kt, seen.lo, seen.hi, lane);
       }
       if (a.direct) {
         const Fold f = fold(M, L, m, l[0][0]);
@@ -759,7 +733,7 @@ __global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
     }
   };
 
-  int t = 0, tn = 0;
+  int t = 0, tn = 0, odd_tiles = 0;  // odd_tiles: of the chunk, a bit each
   // One tile out of (kb, vb), buffer buf.  EDGE: some row does not see it whole.
   auto work = [&](auto edge, const T* kb, const T* vb, int buf) {
     constexpr bool EDGE = decltype(edge)::value;
@@ -794,25 +768,23 @@ __global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
         for (int nb = 0; nb < NB; ++nb) O[cb][nb] *= al[cb];
       }
     }
-    u32x4 P[CB][ST];
+    u32x4 P[ST][CB];
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
-      for (int s = 0; s < ST; ++s) P[cb][s] = step_weights<T, BIAS>(a, S[cb], s, m[cb]);
+      for (int s = 0; s < ST; ++s) P[s][cb] = step_weights<T, BIAS>(a, S[cb], s, m[cb]);
 #pragma unroll
     for (int s = 0; s < ST; ++s) {
-      u32x4 v[NB], Ps[CB];
+      u32x4 v[NB];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) v[nb] = v_operand<T, HD>(vb, s, nb, lane);
-#pragma unroll
-      for (int cb = 0; cb < CB; ++cb) Ps[cb] = P[cb][s];
-      step_pv<T, CB, NB>(O, l, Ps, v);
+      step_pv<T, CB, NB>(O, l, P[s], v);
     }
     if (EDGE && all.mixed(k0, LO, HI)) {
       int found = 0;
 #pragma unroll
       for (int w = 0; w < NW; ++w) found |= odd[buf][w];
-      if (__builtin_amdgcn_readfirstlane(found)) add_odd<T, HD, CB, NB>(a, tile.b, hk, O, P, 0, r, k0, LO, HI, lane);
+      odd_tiles |= (__builtin_amdgcn_readfirstlane(found) != 0) << (t & (TPC - 1));
     }
   };
   // Before the workgroup meets over tile t in buffer buf: the rows that this wave loaded.
@@ -825,6 +797,8 @@ __global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
     if (lane == 0) odd[buf][wave] = any;
   };
   auto end_chunk = [&]() {
+    for (; odd_tiles; odd_tiles &= odd_tiles - 1)
+      add_odd<T, HD, CB, NB>(a, tile.b, hk, O, 0, r, (t / TPC * TPC + __builtin_ctz(odd_tiles)) * TILE, LO, HI, lane);
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {
       if (a.direct) {
