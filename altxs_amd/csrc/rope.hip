@@ -281,7 +281,7 @@ extern "C" int32_t altxs_rope(const AltxsRopeArgs* a, altxs_stream_t stream) {
   p.by_token = fast_div(p.u.total * a->H);
   p.tpb = (int)p.by_token.d >= THREADS ? 1 : THREADS / (int)p.by_token.d;
   const int64_t wgs = (a->T + p.tpb - 1) / p.tpb;
-  ALTXS_REQUIRE(wgs < (1ll << 31), "altxs_rope: T=%lld", (long long)a->T);
+  ALTXS_REQUIRE(wgs < (1ll << 24), "altxs_rope: T=%lld", (long long)a->T);  // 2^32 threads a launch
   const dim3 grid((unsigned)wgs);
   BY_TYPE(rope_kernel, a->dtype, vec, inter, grid, (hipStream_t)stream, p);
   ALTXS_CHECK_HIP(hipGetLastError());
@@ -337,7 +337,9 @@ extern "C" int32_t altxs_paged_append(const AltxsPagedAppendArgs* a, altxs_strea
   p.by_token = fast_div(p.u.total * (p.Hq + 2 * p.Hkv));
   p.tpb = (int)p.by_token.d >= THREADS ? 1 : THREADS / (int)p.by_token.d;
   if (p.tpb > MAX_TPB) p.tpb = MAX_TPB;
-  const dim3 grid((unsigned)((a->T + p.tpb - 1) / p.tpb));
+  const int64_t wgs = (a->T + p.tpb - 1) / p.tpb;
+  ALTXS_REQUIRE(wgs < (1ll << 24), "altxs_paged_append: T=%lld", (long long)a->T);
+  const dim3 grid((unsigned)wgs);
   BY_TYPE(append_kernel, a->dtype, vec, inter, grid, (hipStream_t)stream, p);
   ALTXS_CHECK_HIP(hipGetLastError());
   return ALTXS_OK;

@@ -441,8 +441,8 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
                softcap: float = 0.0, slopes: torch.Tensor | None = None, window: int = 0,
                starts: torch.Tensor | None = None, prefix: torch.Tensor | None = None,
                out: torch.Tensor | None = None, err: torch.Tensor | None = None) -> torch.Tensor:
-    """Attention of the new tokens q [T, H, hd] (hd 64 or 128) over their segments'
-    pages, in which their own keys and values already are (:func:`paged_append`
+    """Attention of the new tokens q [T, H, hd] (hd 64 or 128; fp32, bf16 or fp16; rows
+    of q and the caches at multiples of 16 bytes) over their segments' pages, in which their own keys and values already are (:func:`paged_append`
     with the same table, pos and cu); H a multiple of the cache's heads.
 
     The token at position p sees the keys [lo, hi): hi = p + 1, or the first
@@ -469,6 +469,9 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
         os_ = (H * hd, hd)
     else:
         os_ = _output(out, "out", q, q)
+    max_len = min(width * page, 2**31 - 1) if max_len is None else max_len
+    if not (0 <= max_len < 2**31 and 0 <= window < 2**31):
+        raise ValueError(f"max_len={max_len} and window={window} must be 0 to 2^31 - 1")
     if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (H,) or slopes.get_device() != index
                                or not slopes.is_contiguous()):
         raise ValueError(f"slopes must be a contiguous fp32 tensor [{H}] on device {index}")
@@ -477,7 +480,7 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
                            _index(prefix, "prefix", B, index) if prefix is not None else None,
                            slopes.data_ptr() if slopes is not None else None, _err(err, index), None, 0, T, n_pages,
                            qs[0], qs[1], os_[0], os_[1], kv[0], kv[1], kv[2], hd ** -0.5 if scale is None else scale, softcap,
-                           B, H, Hkv, hd, page, width, width * page if max_len is None else max_len, window, _DT[dtype])
+                           B, H, Hkv, hd, page, width, max_len, window, _DT[dtype])
     n = _lib.load().altxs_paged_attn_workspace_bytes(ctypes.byref(a))
     if n:
         if n < 0:

@@ -139,6 +139,12 @@ def test_bits_do_not_depend_on_the_call(dtype, hd):
         for a, b in ((0, 5), (250, 270), (500, 564), (123, 700)):
             win = dict(q=c["q"][a:b], k=c["k"], v=c["v"], table=c["table"], pos=torch.tensor([a], dtype=torch.int32))
             assert torch.equal(_bits(_run(win, **masks)), _bits(whole[a:b])), (a, b)
+        # a bound of 16384 keys: the chunks are shared among workgroups and folded by a second launch
+        far = torch.full((1, 256), -1, dtype=torch.int32)
+        far[:, :c["table"].shape[1]] = c["table"]
+        for a, b in ((0, 1), (699, 700), (250, 253), (100, 700)):
+            win = dict(q=c["q"][a:b], k=c["k"], v=c["v"], table=far, pos=torch.tensor([a], dtype=torch.int32))
+            assert torch.equal(_bits(_run(win, **masks)), _bits(whole[a:b])), (a, b)
         # many windows in one call: enough work that the keys are not split
         many = dict(q=c["q"][:640], k=c["k"], v=c["v"], table=c["table"].expand(640 // 16, -1).contiguous(),
                     pos=torch.arange(0, 640, 16, dtype=torch.int32))
@@ -309,8 +315,12 @@ def test_refuses():
                dict(out=d["q"][:, :1].expand(4, 4, 64)), dict(err=i32(1).long())):
         with pytest.raises(ValueError):
             ops.paged_attn(**{**ok, **kw})
-    for kw in (dict(max_len=1 << 20), dict(scale=0.0), dict(scale=-1.0), dict(softcap=-1.0), dict(window=-2),
-               dict(q=d["q"][:, :3]), dict(max_len=-1)):
+    for kw in (dict(max_len=-1), dict(window=-2), dict(window=1 << 31), dict(max_len=1 << 40), dict(window=(1 << 32) + 1)):
+        with pytest.raises(ValueError):
+            ops.paged_attn(**{**ok, **kw})
+    odd = torch.zeros(4 * 4 * 64 + 1, dtype=BF, device=DEV)[1:].view(4, 4, 64)
+    for kw in (dict(max_len=1 << 20), dict(scale=0.0), dict(scale=-1.0), dict(softcap=-1.0), dict(q=d["q"][:, :3]),
+               dict(q=odd), dict(out=odd)):
         with pytest.raises(RuntimeError):
             ops.paged_attn(**{**ok, **kw})
     assert ops.paged_attn(**{**ok, "q": d["q"][:0], "cu": i32(3)}).shape == (0, 4, 64)
