@@ -4,10 +4,8 @@
 //   y = softmax(s) V,  s_key = bias(scale q . k_key),  key in [lo, hi)
 //
 // The softmax in one pass.  Keys come in tiles of 64 and chunks of 4 tiles.
-// Inside a chunk a running maximum m, sum l and output O are kept over the
-// tiles (m moves only when a tile's maximum passes it by more than 8 powers of
-// two, so O is rarely rescaled; weights stay below 2^8); a chunk starts afresh,
-// and the chunks' (m, l, O) are folded in order:
+// Inside a chunk a running maximum m, sum l and output O are kept over the tiles; a
+// chunk starts afresh, and the chunks' (m, l, O) are folded in order:
 //   M' = max(M, m), L' = L 2^(M - M') + l 2^(m - M'), O likewise.
 // Tiles and chunks begin at multiples of their sizes from key 0, so a row's
 // arithmetic is the same wherever its chunks are worked on -- one after the
@@ -24,6 +22,14 @@
 // in that order comes out of row-major V tiles in LDS by ds_read_b64_tr_b16.
 // Rows of a tile are (token, query head of the kv head's group) pairs, token-major:
 // grouped heads and neighbouring tokens share every K and V read.
+//
+// Rounding.  In the 16-bit types the weights 2^(s - m) go into the P V products rounded to
+// the type, and l sums the rounded ones.  The largest of a tile that moves m is one,
+// exactly: m follows every tile's maximum for that (letting it trail by up to 8 powers of
+// two, so that O is rescaled less often, saves 4% of chunk scoring and costs a third
+// of the accuracy: error against 64 bits 1.25 to 1.4 times that of fp32 weights and a
+// rounded output, against 1.07; a second product with the remainders would make it 1.0
+// and chunk scoring 27% slower).  Everything else is fp32.
 //
 // Two kernels, one arithmetic:
 //   few   up to 16 rows a segment and kv head on average (decode): 16-row tiles.  A
@@ -53,7 +59,6 @@ using namespace altxs_paged;
 constexpr int THREADS = 256, WAVES = THREADS / WAVE, TILE = 64, CHUNK = 256, TPC = CHUNK / TILE;
 static_assert(TPC == WAVES, "the few-row kernel gives each wave a tile of the chunk");
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LAZY = 8.f;  // how far (powers of two) a tile's maximum passes m before m moves
 
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__bf16 x) { return (float)x; }
@@ -312,7 +317,7 @@ __device__ __forceinline__ void tile_scores(const AttnP& a, f32x4 (&S)[CB][4], f
 __device__ __forceinline__ float next_max(float& m, float mx) {
 #pragma clang fp contract(off)
   const float old = m;
-  m = mx > old + LAZY ? mx : old;
+  m = fmaxf(old, mx);
   return m == old ? 1.f : __builtin_amdgcn_exp2f(old - m);
 }
 
@@ -608,8 +613,11 @@ __device__ __forceinline__ int many_slot(const AttnP& a, int i, int& hk) {
   return (pair - hk * a.B + 1) * (int)a.by_tiles.d - 1 - back;
 }
 
+// (the largest instance would leave its lambdas as calls, their captures in scratch memory)
+#define ALTXS_INLINE __attribute__((always_inline))
+
 template <class T, int HD, bool BIAS>
-__global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
+__global__ __launch_bounds__(NW* WAVE, HD * sizeof(T) > 256 ? 1 : 2) void attn_many_kernel(AttnP a) {
 #pragma clang fp contract(off)
   constexpr int CB = many_cb<T, HD>, MANY = many_rows<T, HD>, EL = Op<T>::EL, KS = HD / (4 * EL), ST = STEPS<T>, NB = HD / 16;
   constexpr int PR = PIECES<T, HD>, RPW = WAVE / PR, RPL = NW * RPW, LOADS = TILE / RPL;  // rows of a wave's load, of the workgroup's; loads
@@ -672,7 +680,7 @@ __global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
   // read for the nearest tile or key of the union (inside the table).
   const const_i32* entries = (const const_i32*)(a.table + (int64_t)tile.b * a.width);
   const bool large = a.shift >= 6;
-  auto lookup = [&](int t, int (&e)[LOADS]) {
+  auto lookup = [&](int t, int (&e)[LOADS]) ALTXS_INLINE {
     if (large) {
       const int entry = entries[(t < t_end ? t : t_end - 1) >> (a.shift - 6)];
 #pragma unroll
@@ -697,7 +705,7 @@ __global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
     vl[i] = (const T*)a.v + hk * a.kv_head + (uint64_t)krow * a.kv_slot + EL * v_piece<T, HD>(krow + i * RPL, lane % PR);
   }
   const uint64_t down = RPL * (uint64_t)a.kv_slot;  // a load's rows to the next one's
-  auto load = [&](int t, const int (&e)[LOADS], T* kb, T* vb) {
+  auto load = [&](int t, const int (&e)[LOADS], T* kb, T* vb) ALTXS_INLINE {
     const bool whole = (uint32_t)(t - whole0) < wholes;
     if (large && whole && (uint32_t)e[0] < n_pages) {
       uint64_t at = (uint64_t)(uint32_t)e[0] * a.kv_page + (uint64_t)(uint32_t)((t << 6) & ((1 << a.shift) - 1)) * a.kv_slot;
@@ -735,7 +743,7 @@ __global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
 
   int t = 0, tn = 0, odd_tiles = 0;  // odd_tiles: of the chunk, a bit each
   // One tile out of (kb, vb), buffer buf.  EDGE: some row does not see it whole.
-  auto work = [&](auto edge, const T* kb, const T* vb, int buf) {
+  auto work = [&](auto edge, const T* kb, const T* vb, int buf) ALTXS_INLINE {
     constexpr bool EDGE = decltype(edge)::value;
     const int k0 = t * TILE;
     if (EDGE && !(seen.lo < k0 + TILE && seen.hi > k0)) return;  // no row of the wave sees any of it
@@ -788,7 +796,7 @@ __global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
     }
   };
   // Before the workgroup meets over tile t in buffer buf: the rows that this wave loaded.
-  auto clean = [&](int t, T* vb, int buf) {
+  auto clean = [&](int t, T* vb, int buf) ALTXS_INLINE {
     if (!all.mixed(t * TILE, LO, HI)) return;
     bool found = false;
 #pragma unroll
@@ -796,7 +804,7 @@ __global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
     const bool any = __any(found);
     if (lane == 0) odd[buf][wave] = any;
   };
-  auto end_chunk = [&]() {
+  auto end_chunk = [&]() ALTXS_INLINE {
     for (; odd_tiles; odd_tiles &= odd_tiles - 1)
       add_odd<T, HD, CB, NB>(a, tile.b, hk, O, 0, r, (t / TPC * TPC + __builtin_ctz(odd_tiles)) * TILE, LO, HI, lane);
 #pragma unroll
@@ -823,7 +831,7 @@ __global__ __launch_bounds__(NW* WAVE, 2) void attn_many_kernel(AttnP a) {
   // (kn, vn), and the entries of the one after it are read; false after the last.
   int en[LOADS];
   const uint32_t n_in = in1 > in0 ? in1 - in0 : 0;
-  auto step = [&](const T* kb, const T* vb, T* kn, T* vn, int buf) {
+  auto step = [&](const T* kb, const T* vb, T* kn, T* vn, int buf) ALTXS_INLINE {
     if (tn < t_end) load(tn, en, kn, vn);
     const int tnn = after(tn);
     lookup(tnn, en);
