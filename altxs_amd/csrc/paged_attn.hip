@@ -996,10 +996,10 @@ static int32_t check(const AltxsPagedAttnArgs* a, const char* who) {
                 who, a->H, a->Hkv);
   ALTXS_REQUIRE(a->page_size >= 16 && a->page_size <= 1024 && (a->page_size & (a->page_size - 1)) == 0,
                 "%s: page_size=%d must be a power of two from 16 to 1024", who, a->page_size);
-  ALTXS_REQUIRE(a->T >= 0 && a->T * a->H < (1ll << 31) && a->B >= 0 && a->n_pages >= 0 && a->table_width >= 0,
+  ALTXS_REQUIRE(a->T >= 0 && a->T < (1ll << 31) && a->T * a->H < (1ll << 31) && a->B >= 0 && a->n_pages >= 0 && a->table_width >= 0,
                 "%s: bad T, B, n_pages or table_width", who);
-  ALTXS_REQUIRE(a->max_len >= 0 && a->max_len <= (int64_t)a->table_width * a->page_size,
-                "%s: max_len=%d is more than table_width * page_size", who, a->max_len);
+  ALTXS_REQUIRE(a->max_len >= 0 && a->max_len <= (int64_t)a->table_width * a->page_size && a->max_len <= 1 << 30,
+                "%s: max_len=%d is more than table_width * page_size or 2^30", who, a->max_len);
   for (int64_t st : {a->kv_page, a->kv_head, a->kv_slot})
     ALTXS_REQUIRE(st >= 0 && st < (1ll << 31), "%s: a cache stride of %lld elements", who, (long long)st);
   ALTXS_REQUIRE(a->scale > 0.f && a->scale < INFINITY, "%s: scale=%g must be positive", who, a->scale);
@@ -1021,6 +1021,8 @@ extern "C" int32_t altxs_paged_attn(const AltxsPagedAttnArgs* a, altxs_stream_t 
   if (a->T == 0 || a->B == 0) return ALTXS_OK;
   ALTXS_REQUIRE(a->q && a->out && a->k_cache && a->v_cache && a->table && a->pos, "altxs_paged_attn: null pointer");
   const Plan pl = plan_of(a);
+  // 2^32 threads a launch; also B * Hkv < 2^24, as each segment has a tile
+  ALTXS_REQUIRE(pl.wgs < (1ll << 24), "altxs_paged_attn: too many row tiles (T=%lld, B=%d)", (long long)a->T, a->B);
   uintptr_t bits = (uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)a->k_cache | (uintptr_t)a->v_cache;
   for (int64_t st : {a->q_tok, a->q_head, a->out_tok, a->out_head, a->kv_page, a->kv_head, a->kv_slot})
     bits |= (uintptr_t)(st * (a->dtype == ALTXS_F32 ? 4 : 2));
@@ -1052,7 +1054,6 @@ extern "C" int32_t altxs_paged_attn(const AltxsPagedAttnArgs* a, altxs_stream_t 
     if (a->head_dim == 64) hipLaunchKernelGGL((K<T, 64, ##__VA_ARGS__>), grid, block, 0, s, p);  \
     else hipLaunchKernelGGL((K<T, 128, ##__VA_ARGS__>), grid, block, 0, s, p);       \
   } while (0)
-  ALTXS_REQUIRE(pl.wgs < (1ll << 24), "altxs_paged_attn: too many row tiles");  // 2^32 threads a launch
   auto go = [&](auto t) {
     using T = decltype(t);
     dim3 grid((unsigned)pl.wgs, (unsigned)pl.split);

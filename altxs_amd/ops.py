@@ -272,21 +272,34 @@ def _span(t: torch.Tensor) -> tuple[int, int]:
     return lo, lo + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
 
 
+def _apart(t: torch.Tensor, x: torch.Tensor) -> bool:
+    """Whether two [T, heads, head_dim] tensors share no memory: their spans do not meet, or
+    their tokens alternate in one buffer (q, k and v as parts of one array)."""
+    lo, hi = _span(t)
+    xl, xh = _span(x)
+    if hi <= xl or xh <= lo:
+        return True
+    size, period = t.element_size(), t.stride(0) * t.element_size()
+    if x.stride(0) != t.stride(0) or not period:
+        return False
+    d = (xl - lo) % period
+    width, xwidth = (size * (1 + (n[1] - 1) * st[1] + n[2] - 1) for n, st in ((t.shape, t.stride()), (x.shape, x.stride())))
+    return d >= width and d + xwidth <= period
+
+
 def _output(t: torch.Tensor, name: str, like: torch.Tensor, *reads: torch.Tensor) -> tuple:
-    """Strides of a caller's output: ``like``'s shape, every element its own, and each tensor that
-    is read either the output itself or apart from it."""
+    """Strides of a caller's output: ``like``'s shape, every element its own, and either ``like``
+    itself or apart from it, and apart from the other tensors that are read."""
     st = _heads(t, name, like.get_device(), like.dtype)
     if t.shape != like.shape:
         raise ValueError(f"{name} must have the shape {tuple(like.shape)}")
     if any(n > 1 and s == 0 for n, s in zip(t.shape, st)):
         raise ValueError(f"{name} must not be expanded")
     if t.numel():
-        lo, hi = _span(t)
-        for x in reads:
-            if x.numel() and not (x.data_ptr() == lo and x.stride() == st):
-                xl, xh = _span(x)
-                if lo < xh and xl < hi:
-                    raise ValueError(f"{name} must be the input itself or not overlap it")
+        for x in (like, *reads):
+            same = x is like and x.data_ptr() == t.data_ptr() and x.stride() == st
+            if x.numel() and not same and not _apart(t, x):
+                raise ValueError(f"{name} must be the input itself or not overlap what is read")
     return st
 
 
@@ -348,7 +361,7 @@ def rope(x: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, sin: torch.Tenso
         out = torch.empty((T, H, hd), dtype=x.dtype, device=x.device)
         os_ = (H * hd, hd)
     else:
-        os_ = _output(out, "out", x, x)
+        os_ = _output(out, "out", x)
     a = _lib.RopeArgs(x.data_ptr(), out.data_ptr(), _index(pos, "pos", T, index), cos.data_ptr(), sin.data_ptr(),
                       _err(err, index), T, rows, xs[0], xs[1], os_[0], os_[1], H, hd, rot, _DT[x.dtype],
                       (_lib.ROPE_INTERLEAVED if interleaved else 0) | (_lib.ROPE_INVERSE if inverse else 0))
@@ -422,7 +435,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
                 result = torch.empty((T, H, hd), dtype=dtype, device=q.device)
                 os_ = (H * hd, hd)
             else:
-                result, os_ = q_out, _output(q_out, "q_out", q, q, k, v)
+                result, os_ = q_out, _output(q_out, "q_out", q, k, v)
             if H:
                 qp, qo = q.data_ptr(), result.data_ptr()
     elif q_out is not None:
@@ -468,9 +481,9 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
         out = torch.empty((T, H, hd), dtype=dtype, device=q.device)
         os_ = (H * hd, hd)
     else:
-        os_ = _output(out, "out", q, q)
-    max_len = min(width * page, 2**31 - 1) if max_len is None else max_len
-    if not (0 <= max_len < 2**31 and 0 <= window < 2**31):
+        os_ = _output(out, "out", q)
+    max_len = min(width * page, 2**30) if max_len is None else max_len
+    if not (0 <= max_len < 2**31 and 0 <= window < 2**31):  # what the structure's fields hold
         raise ValueError(f"max_len={max_len} and window={window} must be 0 to 2^31 - 1")
     if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (H,) or slopes.get_device() != index
                                or not slopes.is_contiguous()):

@@ -689,7 +689,8 @@ int32_t altxs_paged_append(const AltxsPagedAppendArgs *a, altxs_stream_t stream)
  * row's own query, keys and masks alone -- not on the batch, the chunk it came
  * in, the pages or the launch -- so encode windows and decode rows agree.
  *
- * max_len bounds the keys of a segment (at most table_width * page_size); it
+ * Rows of q, out and the caches start at multiples of 16 bytes (strides too).
+ * max_len bounds the keys of a segment (at most table_width * page_size and 2^30); it
  * sizes the launch, so pass the real bound when it is known.  ws:
  * altxs_paged_attn_workspace_bytes(a) bytes, 16-byte aligned, not shared by calls that
  * may overlap.  Replaces run_split_attn / _static_window_attention

@@ -271,6 +271,22 @@ def test_append_layouts():
     assert torch.equal(_bits(odd), _bits(kc))
 
 
+def test_append_in_place_in_a_packed_array():
+    """q, k and v as parts of one [T, H + 2 Hkv, hd] array, q rotated where it lies."""
+    from altxs_amd import ops
+
+    q, k, v, kc, vc, table, pos, cu = _append_case([2, 5], [0, 30], 4, 2, 64, 16, torch.bfloat16, 8)
+    cos, sin = _tables(64, 16)
+    kc2, vc2 = kc.clone(), vc.clone()
+    want = ops.paged_append(k, v, kc, vc, table, pos, cu=cu, q=q, cos=cos, sin=sin)
+    qkv = torch.cat([q, k, v], 1)
+    parts = qkv[:, :4], qkv[:, 4:6], qkv[:, 6:]
+    got = ops.paged_append(parts[1], parts[2], kc2, vc2, table, pos, cu=cu, q=parts[0], q_out=parts[0], cos=cos, sin=sin)
+    assert got.data_ptr() == qkv.data_ptr() and torch.equal(_bits(got), _bits(want))
+    assert torch.equal(_bits(kc2), _bits(kc)) and torch.equal(_bits(vc2), _bits(vc))
+    assert torch.equal(_bits(parts[1]), _bits(k)) and torch.equal(_bits(parts[2]), _bits(v))
+
+
 def test_append_flags():
     """Bad pages, positions and cu: flagged, the rest appended, nothing else touched."""
     from altxs_amd import ops
@@ -313,6 +329,7 @@ def test_append_refuses():
                dict(v_cache=vc[:, :, :8]), dict(table=table.long()), dict(table=table[0]), dict(table=table.t()),
                dict(pos=pos.long()), dict(pos=pos[:1]), dict(cu=cu[:2]), dict(cos=None), dict(q=q[:1]), dict(q=q.half()),
                dict(q_out=q[:, :2]), dict(q_out=k[:, :1].expand(4, 4, 64)), dict(cos=None, sin=None, q_out=q),
+               dict(q=q[:, :2], q_out=k), dict(q=q[:, :2], q_out=v), dict(q=q[:, :2], q_out=q[:, 1:3]),
                dict(k=k[:3], v=v[:3], q=q[:3], cu=None), dict(pos=pos.cpu())):
         with pytest.raises(ValueError):
             ops.paged_append(**{**ok, **kw})

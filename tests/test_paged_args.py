@@ -76,7 +76,8 @@ def test_append_refusals(kw, what):
     (dict(page_size=100), b"page_size"), (dict(max_len=129), b"max_len"), (dict(scale=0.0), b"scale"),
     (dict(scale=-1.0), b"scale"), (dict(scale=float("nan")), b"scale"), (dict(softcap=-1.0), b"softcap"),
     (dict(softcap=float("inf")), b"softcap"), (dict(window=-1), b"window"), (dict(T=5), b"equal segments"),
-    (dict(T=1 << 29), b"bad T"), (dict(kv_slot=-64), b"stride"), (dict(kv_page=1 << 31), b"stride"), (dict(q=None), b"null"), (dict(pos=None), b"null"),
+    (dict(T=1 << 29), b"bad T"), (dict(T=1 << 62), b"bad T"), (dict(table_width=1 << 25, max_len=(1 << 30) + 1), b"max_len"),
+    (dict(B=1 << 29, cu=FAKE), b"row tiles"), (dict(B=(1 << 31) - 1, H=4096, Hkv=4096, cu=FAKE), b"row tiles"), (dict(kv_slot=-64), b"stride"), (dict(kv_page=1 << 31), b"stride"), (dict(q=None), b"null"), (dict(pos=None), b"null"),
 ])
 def test_attn_refusals(kw, what):
     L = _lib.load()
@@ -104,6 +105,22 @@ def test_struct_layouts(tmp_path):
     out = subprocess.run([str(tmp_path / "layout")], capture_output=True, text=True, check=True).stdout.split()
     want = [n for py in names.values() for n in [ctypes.sizeof(py)] + [getattr(py, f[0]).offset for f in py._fields_]]
     assert [int(x) for x in out] == want
+
+
+def test_apart():
+    """Which outputs share memory with an input: against the sets of elements."""
+    buf = torch.arange(6 * 10 * 4)
+    def view(off, T, H, st):
+        return buf.as_strided((T, H, 4), (st, 4, 1), off)
+    views = [view(o, T, H, st) for o in (0, 4, 8, 16, 40, 60, 120) for T in (1, 3) for H in (1, 2) for st in (8, 12, 40)]
+    for t in views:
+        for x in views:
+            if ops._apart(t, x):
+                assert not set(t.flatten().tolist()) & set(x.flatten().tolist())
+    packed = buf[:240].view(6, 10, 4)
+    q, k, v = packed[:, :6], packed[:, 6:8], packed[:, 8:]
+    assert all(ops._apart(a, b) for a in (q, k, v) for b in (q, k, v) if a is not b)
+    assert not ops._apart(q, q) and not ops._apart(packed[:, :7], k) and not ops._apart(k, packed[1:, 7:])
 
 
 def test_host_tensors_are_refused():
