@@ -76,10 +76,35 @@ ALTXS_HD int32_t page_of(const int32_t* row, int32_t width, int32_t shift, int64
   return g < 0 || g >= n_pages ? -1 : g;
 }
 
+// Segments lo .. lo + n - 1 in 64 parts: the last segment of part `lane` (its own, or that of
+// the last part that has any), and the first part whose bit is set (else the last).
+struct Block {
+  int32_t lo, n;
+};
+ALTXS_HD int32_t part_end(const Block b, int lane) {
+  const int64_t end = (int64_t)(lane + 1) * ((b.n - 1) / 64 + 1);
+  return b.lo + (int32_t)(end < b.n ? end : b.n) - 1;
+}
+ALTXS_HD Block part_of(const Block b, uint64_t bits) {
+  const int32_t step = (b.n - 1) / 64 + 1, k = bits ? __builtin_ctzll(bits) : (b.n - 1) / step, left = b.n - k * step;
+  return Block{b.lo + k * step, left < step ? left : step};
+}
+
 #if defined(__HIPCC__)
-// The segment of token t, asked by a whole wave: 64 segments per step, each lane with
-// one's bounds and position (so nothing is read again once it is found); -1: the token
-// belongs to nobody.  cu = NULL: every segment has W tokens.
+// The first of a block of at most 64 segments that holds the first one of which `later` holds,
+// asked by a whole wave: two steps serve 4096 segments.  `later` is false, then true, when cu
+// ascends; with any other cu some block comes out.
+// (Decoding 4096 ragged segments of 100 keys takes 219 us, equal ones, which need no
+// search, 186; 64 segments after the other it took 532.)
+template <class F> __device__ __forceinline__ int block_with_first(int B, int lane, F later) {
+  Block b = {0, B};
+  while (b.n > 64) b = part_of(b, __ballot(later(part_end(b, lane))));
+  return b.lo;
+}
+
+// The segment of token t, asked by a whole wave, each lane with one's bounds and position (so
+// nothing is read again once it is found); -1: the token belongs to nobody.  cu = NULL: every
+// segment has W tokens.
 __device__ __forceinline__ int token_segment(const int32_t* cu, const int32_t* pos, int B, int W, int64_t t, int64_t T, int cap,
                                              int lane, Segment& s) {
   if (!cu) {
@@ -87,15 +112,14 @@ __device__ __forceinline__ int token_segment(const int32_t* cu, const int32_t* p
     s = segment_of(b * W, b * W + W, pos[b], T, cap);
     return b;
   }
-  for (int i = 0; i < B; i += 64) {
-    const int j = i + lane < B ? i + lane : B - 1;
-    const int c0 = cu[j], c1 = cu[j + 1], p = pos[j];
-    const uint64_t later = __ballot(i + lane < B && c1 > t);
-    if (later) {
-      const int l = __builtin_ctzll(later);
-      s = segment_of(__builtin_amdgcn_readlane(c0, l), __builtin_amdgcn_readlane(c1, l), __builtin_amdgcn_readlane(p, l), T, cap);
-      return i + l;
-    }
+  const int i = block_with_first(B, lane, [&](int j) { return cu[j + 1] > t; });
+  const int j = i + lane < B ? i + lane : B - 1;
+  const int c0 = cu[j], c1 = cu[j + 1], p = pos[j];
+  const uint64_t later = __ballot(i + lane < B && c1 > t);
+  if (later) {
+    const int l = __builtin_ctzll(later);
+    s = segment_of(__builtin_amdgcn_readlane(c0, l), __builtin_amdgcn_readlane(c1, l), __builtin_amdgcn_readlane(p, l), T, cap);
+    return i + l;
   }
   s = Segment{0, 0, 0, 0};
   return -1;

@@ -93,10 +93,10 @@ struct RowTile {
   Segment s;
 };
 
-// Which tile slot `slot` is, of `br` rows; every wave finds it for itself, 64
-// segments per step, each lane with one's bounds and position.  The first workgroup
-// also checks that cu ascends (the search itself is safe with any).
-__device__ __forceinline__ RowTile find_tile(const AttnP& a, int slot, int br, int lane, bool first) {
+// Which tile slot `slot` is, of `br` rows; every wave finds it for itself, each lane with
+// a segment's bounds and position.  One wave of each of the first slots also checks 64 of
+// cu's entries (the search itself is safe with any).
+__device__ __forceinline__ RowTile find_tile(const AttnP& a, int slot, int br, int lane, bool check) {
   RowTile t;
   t.b = a.B;
   t.r0 = t.rows = 0;
@@ -108,21 +108,23 @@ __device__ __forceinline__ RowTile find_tile(const AttnP& a, int slot, int br, i
     t.r0 = (slot - t.b * (int)a.by_tiles.d) * br;
     return t;
   }
-  for (int i = 0; i < a.B; i += WAVE) {
-    const int j = i + lane < a.B ? i + lane : a.B - 1;
-    const int c0 = a.cu[j], c1 = a.cu[j + 1], p = a.pos[j];
-    if (first && __any(c1 < c0 || c1 > a.T || (j == 0 && c0 != 0)) && lane == 0) flag_err(a.err, ALTXS_EDEV_POS);
-    const int e = c1 < 0 ? 0 : c1 > a.T ? (int)a.T : c1;
-    const uint64_t later = __ballot(i + lane < a.B && first_slot(e, a.G, br, j + 1) > slot);
-    if (later && t.b == a.B) {
-      const int n = __builtin_ctzll(later);
-      t.b = i + n;
-      t.s = segment_of(__builtin_amdgcn_readlane(c0, n), __builtin_amdgcn_readlane(c1, n), __builtin_amdgcn_readlane(p, n), a.T, a.cap);
-      const int64_t k = slot - first_slot(t.s.t0, a.G, br, t.b);
-      t.rows = t.s.n * a.G;
-      t.r0 = k < 0 || k * br >= t.rows ? t.rows : (int)(k * br);
-      if (!first) break;
-    }
+  if (check && slot < (a.B + WAVE - 1) / WAVE) {
+    const int j = slot * WAVE + lane < a.B ? slot * WAVE + lane : a.B - 1;
+    const int c0 = a.cu[j], c1 = a.cu[j + 1];
+    if (__any(c1 < c0 || c1 > a.T || (j == 0 && c0 != 0)) && lane == 0) flag_err(a.err, ALTXS_EDEV_POS);
+  }
+  auto end_of = [&](int c1) { return c1 < 0 ? 0 : c1 > a.T ? (int)a.T : c1; };
+  const int i = block_with_first(a.B, lane, [&](int j) { return first_slot(end_of(a.cu[j + 1]), a.G, br, j + 1) > slot; });
+  const int j = i + lane < a.B ? i + lane : a.B - 1;
+  const int c0 = a.cu[j], c1 = a.cu[j + 1], p = a.pos[j];
+  const uint64_t later = __ballot(i + lane < a.B && first_slot(end_of(c1), a.G, br, j + 1) > slot);
+  if (later) {
+    const int n = __builtin_ctzll(later);
+    t.b = i + n;
+    t.s = segment_of(__builtin_amdgcn_readlane(c0, n), __builtin_amdgcn_readlane(c1, n), __builtin_amdgcn_readlane(p, n), a.T, a.cap);
+    const int64_t k = slot - first_slot(t.s.t0, a.G, br, t.b);
+    t.rows = t.s.n * a.G;
+    t.r0 = k < 0 || k * br >= t.rows ? t.rows : (int)(k * br);
   }
   return t;
 }
@@ -484,7 +486,7 @@ __global__ __launch_bounds__(THREADS) void attn_few_kernel(AttnP a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE;
   const int g = lane >> 4, col = lane & 15;
   const int slot = (int)div_by(blockIdx.x, a.by_hkv), hk = blockIdx.x - slot * a.Hkv;
-  const RowTile tile = find_tile(a, slot, 16, lane, blockIdx.x == 0 && blockIdx.y == 0 && wave == 0);
+  const RowTile tile = find_tile(a, slot, 16, lane, hk == 0 && blockIdx.y == 0 && wave == 0);
   if (tile.r0 >= tile.rows) return;
   if (!tile.s.ok && lane == 0) flag_err(a.err, ALTXS_EDEV_POS);
   const Row row[1] = {row_of(a, tile, hk, tile.r0 + col)};
@@ -630,7 +632,7 @@ __global__ __launch_bounds__(NW* WAVE, HD * sizeof(T) > 256 ? 1 : 2) void attn_m
   const int g = lane >> 4, col = lane & 15;
   int hk;
   const int slot = many_slot(a, blockIdx.x, hk);
-  const RowTile tile = find_tile(a, slot, MANY, lane, blockIdx.x == 0 && blockIdx.y == 0 && wave == 0);
+  const RowTile tile = find_tile(a, slot, MANY, lane, hk == 0 && blockIdx.y == 0 && wave == 0);
   if (tile.r0 >= tile.rows) return;
   if (!tile.s.ok && threadIdx.x == 0) flag_err(a.err, ALTXS_EDEV_POS);
   Row r[CB];

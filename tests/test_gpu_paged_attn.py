@@ -67,6 +67,46 @@ def test_causal(shape, dtype):
     _check(paged_case(*shape, dtype, seed=sum(shape[0]) + shape[2]))
 
 
+@pytest.mark.parametrize("B", [65, 300, 5000])
+@pytest.mark.parametrize("n", [1, 40])
+def test_many_ragged_segments(B, n):
+    """Ragged calls search for their segments: the bits of one call per segment, with idle
+    segments between, rows behind the last, and another kernel's tiles."""
+    from altxs_amd import ops
+
+    _log(f"paged_attn ragged B={B} n={n}")
+    g = torch.Generator().manual_seed(B + n)
+    H, Hkv, hd, page = 4, 2, 64, 16
+    if n > 1 and B > 1000:
+        B = 1000
+    lens = torch.randint(0, n + 1, (B,), generator=g) if n > 1 else (torch.rand(B, generator=g) < 0.7).int()
+    cu = torch.cat([torch.zeros(1, dtype=torch.int64), lens.cumsum(0)]).int().to(DEV)
+    T = int(cu[-1]) + 3
+    pos = torch.randint(0, 70, (B,), generator=g, dtype=torch.int32).to(DEV)
+    table = torch.randint(0, 32, (B, 7), generator=g, dtype=torch.int32).to(DEV)
+    kc, vc = (torch.randn(32, Hkv, page, hd, generator=g).to(BF).to(DEV) for _ in range(2))
+    q = torch.randn(T, H, hd, generator=g).to(BF).to(DEV)
+    out = torch.full_like(q, 7.0)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    ops.paged_attn(q, kc, vc, table, pos, cu=cu, out=out, err=err)
+    assert int(err) == 0 and bool((out[T - 3:] == 7).all())
+    # the same tokens as segments of one token each, their positions spelt out: no search
+    seg = torch.repeat_interleave(torch.arange(B), lens.long()).to(DEV)
+    at = torch.arange(T - 3, device=DEV) - cu.long()[seg]
+    one = ops.paged_attn(q[:T - 3], kc, vc, table[seg].contiguous(), (pos[seg] + at).int())
+    assert torch.equal(_bits(out[:T - 3]), _bits(one))
+    # append finds the same places
+    k, v = (torch.randn(T, Hkv, hd, generator=g).to(BF).to(DEV) for _ in range(2))
+    own = torch.arange(B * 7, dtype=torch.int32, device=DEV).view(B, 7)
+    ka, va, kb, vb = (torch.zeros(B * 7, Hkv, page, hd, dtype=BF, device=DEV) for _ in range(4))
+    ops.paged_append(k, v, ka, va, own, pos, cu=cu, err=err)
+    ops.paged_append(k[:T - 3], v[:T - 3], kb, vb, own[seg].contiguous(), (pos[seg] + at).int(), err=err)
+    assert int(err) == 0 and torch.equal(_bits(ka), _bits(kb)) and torch.equal(_bits(va), _bits(vb))
+    cu[B // 2] = T + 9  # one bound past the tokens: flagged, wherever in cu it is
+    ops.paged_attn(q, kc, vc, table, pos, cu=cu, err=err)
+    assert int(err) & 1
+
+
 @pytest.mark.parametrize("dtype", [BF, FP, F32])
 @pytest.mark.parametrize("masks", ["cap", "slopes", "window", "window1", "prefix", "docs", "all"])
 @pytest.mark.parametrize("shape", [SHAPES[4], SHAPES[7], SHAPES[10], SHAPES[12]],

@@ -34,6 +34,23 @@ void t_range(int p, int len, int window, int start, int prefix, int* out) {
   out[0] = r.lo; out[1] = r.hi;
 }
 int t_page(const int* row, int width, int shift, long long n_pages, int t) { return page_of(row, width, shift, n_pages, t); }
+// the block that block_with_first() ends with, when a wave's ballots are `later`
+void t_block(int B, const unsigned char* later, int* out) {
+  Block b = {0, B};
+  out[2] = 0;
+  while (b.n > 64) {
+    unsigned long long m = 0;
+    for (int l = 0; l < 64; ++l) m |= (unsigned long long)later[part_end(b, l)] << l;
+    b = part_of(b, m);
+    ++out[2];
+  }
+  out[0] = b.lo; out[1] = b.n;
+}
+int t_part(int n, unsigned long long bits, int lane, int* out) {
+  const Block b = part_of(Block{0, n}, bits);
+  out[0] = b.lo; out[1] = b.n;
+  return part_end(Block{0, n}, lane);
+}
 }
 """
 
@@ -78,6 +95,28 @@ def test_slots_cover_every_row_once(lib, g, br):
         assert first[-1] <= lib.t_slots(T, g, br, B)
         for b in range(B):
             assert first[b + 1] - first[b] >= -(-int(lens[b]) * g // br)
+
+
+@pytest.mark.parametrize("B", [1, 2, 63, 64, 65, 127, 128, 129, 200, 4095, 4096, 4097, 10000, 300000])
+def test_search_finds_the_first(lib, B):
+    r = np.random.RandomState(B)
+    out = (ctypes.c_int * 3)()
+    for first in sorted({0, 1, 63, 64, 65, B // 2, B - 2, B - 1, *r.randint(0, B, 20).tolist()}):
+        if not 0 <= first < B:
+            continue
+        later = (np.arange(B) >= first).astype(np.uint8)
+        lib.t_block(B, later.ctypes.data_as(ctypes.c_char_p), out)
+        assert 1 <= out[1] <= 64 and 0 <= out[0] <= first < out[0] + out[1] <= B
+        assert 64 ** (out[2] + 1) < 64 * B + 64 * 64
+    for later in (np.zeros(B, np.uint8), (r.rand(B) > 0.5).astype(np.uint8)):  # nobody; no order at all
+        lib.t_block(B, later.ctypes.data_as(ctypes.c_char_p), out)
+        assert 1 <= out[1] <= 64 and 0 <= out[0] and out[0] + out[1] <= B
+    for n in (65, B + 64, (1 << 31) - 1):
+        for lane in (0, 1, 62, 63):
+            end = lib.t_part(n, ctypes.c_ulonglong(1 << lane), lane, out)
+            assert 0 <= end < n
+            if lane * ((n - 1) // 64 + 1) < n:
+                assert out[0] + out[1] - 1 == end and out[1] >= 1
 
 
 def test_segments_stay_in_bounds(lib):
