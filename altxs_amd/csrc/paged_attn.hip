@@ -348,6 +348,7 @@ template <class T, int HD> __device__ __forceinline__ int k_piece(int row, int p
   return piece ^ (PIECES<T, HD> == 8 ? (row >> 1) & 7 : row & 15);
 }
 
+typedef __attribute__((ext_vector_type(2))) uint16_t u16x2;
 typedef __attribute__((__vector_size__(4 * sizeof(short)))) short i16x4;
 typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
 typedef const __attribute__((address_space(1))) void glob_void;
@@ -398,19 +399,37 @@ __device__ __forceinline__ void step_pv(f32x4 (&O)[CB][NB], f32x4 (&l)[CB], cons
   }
 }
 
-// Zero what is not finite in the 16 bytes at `at` (LDS); whether there was any.
-template <class T>
-__device__ __forceinline__ bool take_odd(T* at) {
-  u32x4 v = *(u32x4*)at;
-  uint32_t any = 0;
+// Zero what is not finite in a wave's N loads of V rows (LDS, 64 x 16 bytes each, `step` elements
+// apart); whether any lane found some.  All is read before anything is written, and looked through
+// by the largest magnitude, which is not finite from a full exponent field on.
+template <class T, int N>
+__device__ __forceinline__ bool take_odd(T* at, int step) {
+  constexpr bool W = sizeof(T) == 4;
+  u32x4 v[N];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {  // a full exponent field carries into the bit above it
-    const uint32_t f = ((v[i] & Op<T>::EXP) + Op<T>::ONE) & Op<T>::TOP;
-    any |= f;
-    v[i] &= ~((f << 1) - (f >> (8 * sizeof(T) - 1)));
+  for (int n = 0; n < N; ++n) v[n] = *(const u32x4*)(at + n * step);
+  uint32_t most = 0;
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t mag = v[n][i] & ~Op<T>::TOP;
+      if constexpr (W) most = mag > most ? mag : most;
+      else most = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, mag), __builtin_bit_cast(u16x2, most)));
+    }
+  const bool found = W ? most >= Op<T>::EXP : (most & 0xffff) >= (Op<T>::EXP & 0xffff) || most >= (Op<T>::EXP & 0xffff0000u);
+  if (!__any(found)) return false;
+#pragma unroll 1
+  for (int n = 0; n < N; ++n) {
+    u32x4 x = *(const u32x4*)(at + n * step);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // a full exponent field carries into the bit above it
+      const uint32_t f = ((x[i] & Op<T>::EXP) + Op<T>::ONE) & Op<T>::TOP;
+      x[i] &= ~((f << 1) - (f >> (8 * sizeof(T) - 1)));
+    }
+    *(u32x4*)(at + n * step) = x;
   }
-  if (any) *(u32x4*)at = v;
-  return any != 0;
+  return true;
 }
 
 // What take_odd() took out of tile k0's V, read again from the pages and added to the
@@ -425,14 +444,22 @@ __device__ __forceinline__ void add_odd(const AttnP& a, int b, int hk, f32x4 (&O
     const int entry = key_entry(a, b, key, LO, HI);
     if (entry < 0 || entry >= a.n_pages) continue;
     const T* v = key_row<T>(a.v, entry, key, a.shift, a.kv_page, a.kv_slot, hk * a.kv_head) + 16 * nb0 + 4 * (unhoisted(lane) >> 4);
+    uint32_t in[CB];  // rows that see the key: all ones
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) in[cb] = key >= r[cb].lo && key < r[cb].hi ? ~0u : 0u;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float e = to_f(v[16 * nb + i]);
+        // integers rather than comparisons, whose masks would spill the loop's scalar registers
+        // (packed documents of 128 dims 57 us so, 49 without; the largest dense chunks 125 and 119)
+        const uint32_t e = __float_as_uint(to_f(v[16 * nb + i]));
+        const uint32_t is_odd = (uint32_t)((int32_t)(0x7f7fffffu - (e & 0x7fffffffu)) >> 31);
 #pragma unroll
-        for (int cb = 0; cb < CB; ++cb)
-          if (!(fabsf(e) < INFINITY) && key >= r[cb].lo && key < r[cb].hi) O[cb][nb][i] += e;
+        for (int cb = 0; cb < CB; ++cb) {
+          const uint32_t add = is_odd & in[cb];
+          O[cb][nb][i] += __uint_as_float((e & add) | (0x80000000u & ~add));  // or -0, which changes nothing
+        }
       }
   }
 }
@@ -540,10 +567,7 @@ __global__ __launch_bounds__(THREADS) void attn_few_kernel(AttnP a) {
       for (int s = 0; s < ST; ++s) pt[wave][s][lane] = step_weights<T, BIAS>(a, S[0], s, mw);
       __builtin_amdgcn_s_waitcnt(0);  // the wave's V tile
       if (seen.mixed(k0, seen.lo, seen.hi)) {
-        bool found = false;
-#pragma unroll
-        for (int i = 0; i < TILE / RPL; ++i) found |= take_odd<T>(vt[wave] + i * RPL * HD + EL * lane);
-        const bool any = __any(found);
+        const bool any = take_odd<T, TILE / RPL>(vt[wave] + EL * lane, RPL * HD);
         if (lane == 0) odd[wave] = any;
       }
       __syncthreads();
@@ -749,6 +773,7 @@ __global__ __launch_bounds__(NW* WAVE, HD * sizeof(T) > 256 ? 1 : 2) void attn_m
     constexpr bool EDGE = decltype(edge)::value;
     const int k0 = t * TILE;
     if (EDGE && !(seen.lo < k0 + TILE && seen.hi > k0)) return;  // no row of the wave sees any of it
+    const int found = EDGE ? odd[buf][lane % NW] : 0;  // used at the end, if the tile is mixed
     f32x4 S[CB][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -791,19 +816,13 @@ __global__ __launch_bounds__(NW* WAVE, HD * sizeof(T) > 256 ? 1 : 2) void attn_m
       step_pv<T, CB, NB>(O, l, P[s], v);
     }
     if (EDGE && all.mixed(k0, LO, HI)) {
-      int found = 0;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) found |= odd[buf][w];
-      odd_tiles |= (__builtin_amdgcn_readfirstlane(found) != 0) << (t & (TPC - 1));
+      odd_tiles |= __any(found != 0) << (t & (TPC - 1));
     }
   };
   // Before the workgroup meets over tile t in buffer buf: the rows that this wave loaded.
   auto clean = [&](int t, T* vb, int buf) ALTXS_INLINE {
     if (!all.mixed(t * TILE, LO, HI)) return;
-    bool found = false;
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) found |= take_odd<T>(vb + (i * RPL + wave * RPW) * HD + EL * lane);
-    const bool any = __any(found);
+    const bool any = take_odd<T, LOADS>(vb + wave * RPW * HD + EL * lane, RPL * HD);
     if (lane == 0) odd[buf][wave] = any;
   };
   auto end_chunk = [&]() ALTXS_INLINE {

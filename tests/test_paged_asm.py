@@ -51,6 +51,13 @@ def test_attention_keeps_its_registers(asm):
     assert max(spills.values()) <= 8, {k: v for k, v in spills.items() if v > 8}
 
 
+def test_chunk_loops_keep_their_scalars(asm):
+    """Scalar registers spill into vector lanes, which the loops then read back every tile."""
+    spills = {m[1]: int(m[0]) for m in re.findall(r"\.sgpr_spill_count:\s+(\d+)\s+\.symbol:\s+(\S*attn_many_kernel\S*)\.kd",
+                                                 asm["paged_attn.hip"])}
+    assert len(spills) == 12 and max(spills.values()) <= 12, spills
+
+
 def test_instructions(asm):
     for kernel, wanted in (("attn_many_kernelIDF16bLi64ELb0E", ("ds_read_b64_tr_b16", "global_load_lds_dwordx4",
                                                                "v_mfma_f32_16x16x32_bf16", "s_load_dword")),
