@@ -248,7 +248,7 @@ def rope_tables(length: int, rot: int, base: float = 1e4, *, scaling: str | None
 
 
 # Host time counts here: a decode step's rotation, append or attention runs a few
-# microseconds.  The checks below read each attribute once and build the argument
+# microseconds.  The checks below read each attribute once and pack the argument
 # structure in one call; the stream comes as the handle itself (torch's public
 # current_stream builds an object for it, 1.9 us against 0.1).
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
@@ -311,7 +311,7 @@ def _index(t: torch.Tensor, name: str, n: int, index: int) -> int:
 
 def _err(err: torch.Tensor | None, index: int):
     if err is None:
-        return None
+        return 0
     if err.dtype != torch.int32 or err.get_device() != index or err.numel() < 1:
         raise ValueError(f"err must be an int32 tensor on device {index}")
     return err.data_ptr()
@@ -329,14 +329,14 @@ def _rot_tables(cos: torch.Tensor, sin: torch.Tensor, hd: int, index: int) -> tu
     return rows, 2 * half
 
 
-def _launch(name: str, args, index: int) -> None:
+def _launch(name: str, args: bytes, index: int) -> None:
     """Call ``name`` on the current stream of device ``index`` (which need not be the current one)."""
     f = getattr(_lib.load(), name)
     if index == torch.cuda.current_device():
-        rc = f(ctypes.byref(args), _raw_stream(index))
+        rc = f(args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = f(ctypes.byref(args), _raw_stream(index))
+            rc = f(args, _raw_stream(index))
     if rc:
         _lib.check(rc, name)
 
@@ -362,9 +362,9 @@ def rope(x: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, sin: torch.Tenso
         os_ = (H * hd, hd)
     else:
         os_ = _output(out, "out", x)
-    a = _lib.RopeArgs(x.data_ptr(), out.data_ptr(), _index(pos, "pos", T, index), cos.data_ptr(), sin.data_ptr(),
+    a = _lib.RopeArgs.pack(x.data_ptr(), out.data_ptr(), _index(pos, "pos", T, index), cos.data_ptr(), sin.data_ptr(),
                       _err(err, index), T, rows, xs[0], xs[1], os_[0], os_[1], H, hd, rot, _DT[x.dtype],
-                      (_lib.ROPE_INTERLEAVED if interleaved else 0) | (_lib.ROPE_INVERSE if inverse else 0))
+                      (_lib.ROPE_INTERLEAVED if interleaved else 0) | (_lib.ROPE_INVERSE if inverse else 0), 0)
     if H:
         _launch("altxs_rope", a, index)
     return out
@@ -388,7 +388,7 @@ def _pages(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, po
         return st, B, width, pp, _index(cu, "cu", B + 1, index)
     if B and T % B:
         raise ValueError(f"{T} tokens are not {B} equal segments (give cu)")
-    return st, B, width, pp, None
+    return st, B, width, pp, 0
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor,
@@ -420,7 +420,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin go together")
     rows = rot = H = 0
-    qp = qo = tp = sp = None
+    qp = qo = tp = sp = 0
     qs = os_ = (0, 0)
     result = q
     if cos is not None:
@@ -440,10 +440,10 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
                 qp, qo = q.data_ptr(), result.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out without cos and sin")
-    a = _lib.PagedAppendArgs(k.data_ptr(), v.data_ptr(), qp, qo, k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(),
+    a = _lib.PagedAppendArgs.pack(k.data_ptr(), v.data_ptr(), qp, qo, k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(),
                              pp, cp, tp, sp, _err(err, index), T, n_pages, rows, ks[0], ks[1], vs[0], vs[1],
                              qs[0], qs[1], os_[0], os_[1], kv[0], kv[1], kv[2], B, H, Hkv, hd, page, width, rot,
-                             _DT[dtype], _lib.ROPE_INTERLEAVED if interleaved and rot else 0)
+                             _DT[dtype], _lib.ROPE_INTERLEAVED if interleaved and rot else 0, 0)
     if Hkv:
         _launch("altxs_paged_append", a, index)
     return result
@@ -488,17 +488,23 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
     if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (H,) or slopes.get_device() != index
                                or not slopes.is_contiguous()):
         raise ValueError(f"slopes must be a contiguous fp32 tensor [{H}] on device {index}")
-    a = _lib.PagedAttnArgs(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), table.data_ptr(), pp, cp,
-                           _index(starts, "starts", T, index) if starts is not None else None,
-                           _index(prefix, "prefix", B, index) if prefix is not None else None,
-                           slopes.data_ptr() if slopes is not None else None, _err(err, index), None, 0, T, n_pages,
-                           qs[0], qs[1], os_[0], os_[1], kv[0], kv[1], kv[2], hd ** -0.5 if scale is None else scale, softcap,
-                           B, H, Hkv, hd, page, width, max_len, window, _DT[dtype])
-    n = _lib.load().altxs_paged_attn_workspace_bytes(ctypes.byref(a))
+    def args(ws: int, ws_bytes: int) -> bytes:
+        return _lib.PagedAttnArgs.pack(
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), table.data_ptr(), pp, cp, sp, xp, lp, ep,
+            ws, ws_bytes, T, n_pages, qs[0], qs[1], os_[0], os_[1], kv[0], kv[1], kv[2], scale, softcap,
+            B, H, Hkv, hd, page, width, max_len, window, _DT[dtype], 0)
+
+    sp = _index(starts, "starts", T, index) if starts is not None else 0
+    xp = _index(prefix, "prefix", B, index) if prefix is not None else 0
+    lp = slopes.data_ptr() if slopes is not None else 0
+    ep = _err(err, index)
+    scale = hd ** -0.5 if scale is None else scale
+    a = args(0, 0)
+    n = _lib.load().altxs_paged_attn_workspace_bytes(a)
     if n:
         if n < 0:
             _lib.check(int(n), "altxs_paged_attn")
         ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-        a.ws, a.ws_bytes = ws.data_ptr(), n
+        a = args(ws.data_ptr(), n)
     _launch("altxs_paged_attn", a, index)
     return out

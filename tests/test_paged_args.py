@@ -107,6 +107,14 @@ def test_struct_layouts(tmp_path):
     assert [int(x) for x in out] == want
 
 
+def test_packed_structures():
+    """pack() lays the fields out as the ctypes structure (and so the header) does."""
+    for c in (_lib.RopeArgs, _lib.PagedAppendArgs, _lib.PagedAttnArgs):
+        values = [i / 4 if t is ctypes.c_float else i * 1000003 + 1 for i, (_, t) in enumerate(c._fields_)]
+        got = c.pack(*values)
+        assert len(got) == ctypes.sizeof(c) and got == bytes(c(*values))
+
+
 def test_apart():
     """Which outputs share memory with an input: against the sets of elements."""
     buf = torch.arange(6 * 10 * 4)
