@@ -47,6 +47,7 @@
 // infinities or NaN into a row (0 * inf in P V): in tiles with such keys each wave looks
 // through the V rows it loaded, before the workgroup meets, and zeroes what is not
 // finite; if there was any, it is added to the rows that do see it when the chunk ends.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -987,17 +988,23 @@ Plan plan_of(const AltxsPagedAttnArgs* a) {
   const int br = p.few ? 16 : many(a);
   const int64_t slots = a->cu ? slot_count(a->T, G, br, a->B) : (int64_t)a->B * ((a->T / a->B * G + br - 1) / br);
   p.wgs = slots * a->Hkv;
+  // Row tiles that there are, about: ragged segments' slots are up to B more.
+  int64_t tiles = slots;
+  if (a->cu) tiles = std::max(std::min((int64_t)a->B, a->T), (a->T * G + br - 1) / br);
+  tiles *= a->Hkv;
   // Share a row tile's chunks among workgroups where the row tiles alone do not fill the
   // chip and the time that saves is well above the fold's: a launch, and the partial
   // results written and read at ~3 TB/s.  A workgroup takes ~3.2 us a chunk (few) or
   // ~4.8 (many).  Measured, one against shared: 2 segments decoding at 2048 22.6 / 9.4 us,
   // 48 segments 42.3 / 43.6 (from 384 workgroups on they fill the chip); windows of 512
   // tokens at 8000 163 / 37 us, but chunks of 1024 and 4096 tokens from position 0 24.2 / 23.5
-  // and 81 / 87.
+  // and 81 / 87.  Many rows share no further than one workgroup a place (2 x 256): 1024 took
+  // 40.4 for 37.3 of those windows; 48 drafts of up to 9 tokens 33.7 us counted by their slots and 31.0 by
+  // their tiles.
   const int64_t fill = p.few ? 2048 : 512;
-  if (p.wgs < 384) {
-    int64_t z = (fill + p.wgs - 1) / p.wgs;
-    if (z > p.nc) z = p.nc;
+  if (tiles < 384) {
+    int64_t z = (fill + tiles - 1) / tiles;
+    z = std::max<int64_t>(1, std::min<int64_t>({z, p.nc, 4 * fill / p.wgs}));  // idle segments' workgroups cost their start
     const double chunk_us = p.few ? 3.2 : 4.8;
     const double fold_us = 4.0 + (double)p.rows * p.nc * (a->head_dim + 2) * 8 / 3e6;
     if (p.nc * chunk_us > 1.5 * ((p.nc + z - 1) / z * chunk_us + fold_us)) p.split = (int)z;

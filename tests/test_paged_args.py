@@ -85,6 +85,15 @@ def test_attn_refusals(kw, what):
     assert what in L.altxs_last_error(), L.altxs_last_error()
 
 
+def test_workspace_of_few_tokens_among_many_idle_segments():
+    """Few row tiles share their chunks; hundreds of thousands of idle segments' slots do not multiply by it."""
+    L = _lib.load()
+    big = dict(table_width=512, max_len=32768, cu=FAKE)
+    assert L.altxs_paged_attn_workspace_bytes(ctypes.byref(_attn(B=4, **big))) == 4 * 8 * 128 * (8 + 64 * 4)
+    assert L.altxs_paged_attn_workspace_bytes(ctypes.byref(_attn(B=1000, **big))) == 0
+    assert L.altxs_paged_attn_workspace_bytes(ctypes.byref(_attn(B=1 << 20, **big))) == 0
+
+
 def test_nothing_to_do_is_done():
     L = _lib.load()
     assert L.altxs_rope(ctypes.byref(_rope(T=0, x=None, out=None, pos=None)), None) == 0
