@@ -36,8 +36,8 @@
 //         workgroup takes a chunk at a time, its four waves a tile each for the
 //         scores (K straight into the operand registers) and a quarter of the
 //         dims each for P V, so a chunk's loads are all in flight at once.
-//   many  128-row tiles, 32 rows a wave; K and V tiles go through LDS, loaded
-//         ahead, and are read by all four waves.
+//   many  128-row tiles, 32 rows a wave (64 and 16 for rows of more than 128 bytes); K and
+//         V tiles go through LDS, loaded ahead, and are read by all four waves.
 // fp32 (the framework's exact mode) is the same with v_mfma_f32_16x16x4_f32, 4 keys or dims
 // at a time, exact products and unrounded weights.
 //
@@ -500,6 +500,12 @@ __device__ __forceinline__ void store_part(const AttnP& a, const Row& r, int c, 
 }
 
 // ---- few rows ----------------------------------------------------------------
+//
+// Bound by the cache read.  64 segments decoding at 2048 keys of 8 x 64 bf16 (268 MB): 49 us,
+// 5.5 TB/s; 256 at 4096 (2.1 GB): 359 us, 6.0 TB/s (a large copy moves 5.1, a large read
+// 5.8).  A workgroup has its chunk's 64 KB in flight at once and a CU holds two of them, which
+// is what covers the memory latency; one segment at 2048 is all latency: 5.7 us in 64 workgroups of
+// a chunk each, and the fold's 3.8.
 
 template <class T, int HD, bool BIAS>
 __global__ __launch_bounds__(THREADS) void attn_few_kernel(AttnP a) {
@@ -617,6 +623,13 @@ __global__ __launch_bounds__(THREADS) void attn_few_kernel(AttnP a) {
 }
 
 // ---- many rows ---------------------------------------------------------------
+//
+// Bound by instruction issue: 16 x 2048 new tokens of 8 x 64 bf16 119 us, 577 TFLOP/s (of 1254 that
+// a large product reaches), 128 dims 244 us, 563 TFLOP/s; the matrix cores are busy a
+// quarter of the time and the vector units half of it (a score takes an fma, an exponential,
+// half a conversion and its share of the maximum and the masks), at two waves a SIMD, which
+// the accumulators of a chunk and of the total leave room for.  Eight waves of 16 rows
+// (four a SIMD) spill them: 651 us for 244.  fp32, 4 x 2048: 188 us, 91 TFLOP/s.
 
 constexpr int NW = 4;  // waves of a workgroup
 // 16-row blocks of a wave, and rows of a workgroup
@@ -895,7 +908,9 @@ __global__ __launch_bounds__(NW* WAVE, HD * sizeof(T) > 256 ? 1 : 2) void attn_m
 // One wave per (token, head): a dim (or two) per lane for O, and for each 64 chunks a
 // chunk per lane for the factors -- the running maximum is a prefix maximum, so a
 // scan over the lanes gives the values of fold() for all of them at once.  O is
-// folded in order with the chunks' loads two groups ahead.
+// folded in order with the chunks' loads two groups ahead.  Bound by latency: 512 rows of
+// 128 chunks (17.8 MB) 8.8 us, 1 row of 9 chunks 3.8 us, most of it the start of a launch; factors
+// through LDS or 32 chunks ahead gain nothing (8.2 to 11.3 us).
 template <class T, int HD>
 __global__ __launch_bounds__(THREADS) void attn_fold_kernel(AttnP a) {
 #pragma clang fp contract(off)
