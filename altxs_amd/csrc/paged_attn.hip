@@ -1045,8 +1045,9 @@ static int32_t check(const AltxsPagedAttnArgs* a, const char* who) {
                 "%s: max_len=%d is more than table_width * page_size or 2^30", who, a->max_len);
   for (int64_t st : {a->kv_page, a->kv_head, a->kv_slot})
     ALTXS_REQUIRE(st >= 0 && st < (1ll << 31), "%s: a cache stride of %lld elements", who, (long long)st);
-  ALTXS_REQUIRE(a->scale > 0.f && a->scale < INFINITY, "%s: scale=%g must be positive", who, a->scale);
-  ALTXS_REQUIRE(a->softcap >= 0.f && a->softcap < INFINITY, "%s: softcap=%g", who, a->softcap);
+  ALTXS_REQUIRE(a->scale > 0.f && a->scale * LOG2E < INFINITY, "%s: scale=%g must be positive", who, a->scale);
+  ALTXS_REQUIRE(a->softcap == 0.f || (a->softcap > 0.f && a->softcap * LOG2E < INFINITY && 2.f * (a->scale * LOG2E) / a->softcap < INFINITY),
+                "%s: softcap=%g", who, a->softcap);
   ALTXS_REQUIRE(a->window >= 0, "%s: window=%d", who, a->window);
   ALTXS_REQUIRE(a->T == 0 || a->B == 0 || a->cu || a->T % a->B == 0, "%s: T=%lld tokens are not B=%d equal segments", who,
                 (long long)a->T, a->B);

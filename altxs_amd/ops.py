@@ -358,7 +358,7 @@ def rope(x: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, sin: torch.Tenso
     index = x.get_device()
     rows, rot = _rot_tables(cos, sin, hd, index)
     if out is None:
-        out = torch.empty((T, H, hd), dtype=x.dtype, device=x.device)
+        out = x.new_empty((T, H, hd))
         os_ = (H * hd, hd)
     else:
         os_ = _output(out, "out", x)
@@ -415,7 +415,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
         raise ValueError("k and v must have equal shapes")
     kv, B, width, pp, cp = _pages(k_cache, v_cache, table, pos, cu, T, dtype, index)
     n_pages, ch, page, chd = k_cache.shape
-    if ch != Hkv or chd != hd:
+    if ch != Hkv or chd != hd or not Hkv:
         raise ValueError(f"caches of {ch} heads of {chd}, keys of {Hkv} of {hd}")
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin go together")
@@ -432,7 +432,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
             if qT != T or qd != hd:
                 raise ValueError(f"q must be [{T}, heads, {hd}]")
             if q_out is None:
-                result = torch.empty((T, H, hd), dtype=dtype, device=q.device)
+                result = q.new_empty((T, H, hd))
                 os_ = (H * hd, hd)
             else:
                 result, os_ = q_out, _output(q_out, "q_out", q, k, v)
@@ -444,8 +444,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
                              pp, cp, tp, sp, _err(err, index), T, n_pages, rows, ks[0], ks[1], vs[0], vs[1],
                              qs[0], qs[1], os_[0], os_[1], kv[0], kv[1], kv[2], B, H, Hkv, hd, page, width, rot,
                              _DT[dtype], _lib.ROPE_INTERLEAVED if interleaved and rot else 0, 0)
-    if Hkv:
-        _launch("altxs_paged_append", a, index)
+    _launch("altxs_paged_append", a, index)
     return result
 
 
@@ -478,7 +477,7 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
     if chd != hd:
         raise ValueError(f"caches of heads of {chd}, queries of {hd}")
     if out is None:
-        out = torch.empty((T, H, hd), dtype=dtype, device=q.device)
+        out = q.new_empty((T, H, hd))
         os_ = (H * hd, hd)
     else:
         os_ = _output(out, "out", q)

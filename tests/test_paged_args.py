@@ -75,7 +75,8 @@ def test_append_refusals(kw, what):
     (dict(dtype=-1), b"dtype"), (dict(head_dim=96), b"head_dim"), (dict(H=12), b"multiple"), (dict(Hkv=0), b"multiple"),
     (dict(page_size=100), b"page_size"), (dict(max_len=129), b"max_len"), (dict(scale=0.0), b"scale"),
     (dict(scale=-1.0), b"scale"), (dict(scale=float("nan")), b"scale"), (dict(softcap=-1.0), b"softcap"),
-    (dict(softcap=float("inf")), b"softcap"), (dict(window=-1), b"window"), (dict(T=5), b"equal segments"),
+    (dict(softcap=float("inf")), b"softcap"), (dict(softcap=float("nan")), b"softcap"), (dict(softcap=3e38), b"softcap"),
+    (dict(softcap=1e-40), b"softcap"), (dict(scale=3e38), b"scale"), (dict(window=-1), b"window"), (dict(T=5), b"equal segments"),
     (dict(T=1 << 29), b"bad T"), (dict(T=1 << 62), b"bad T"), (dict(table_width=1 << 25, max_len=(1 << 30) + 1), b"max_len"),
     (dict(B=1 << 29, cu=FAKE), b"row tiles"), (dict(B=(1 << 31) - 1, H=4096, Hkv=4096, cu=FAKE), b"row tiles"), (dict(kv_slot=-64), b"stride"), (dict(kv_page=1 << 31), b"stride"), (dict(q=None), b"null"), (dict(pos=None), b"null"),
 ])
