@@ -356,9 +356,10 @@ typedef const __attribute__((address_space(1))) void glob_void;
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(4))) int32_t const_i32;  // read by scalar loads
 
-// 16 bytes a lane from global memory straight into LDS (lane l's at dst + 16 l).
-__device__ __forceinline__ void load_lds16(const void* src, void* dst) {
-  __builtin_amdgcn_global_load_lds((glob_void*)src, (lds_void*)dst, 16, 0, 0);
+// 16 bytes a lane from global memory straight into LDS (lane l's at dst + 16 l).  ONCE: what
+// nobody reads again soon (the nt bit).
+template <bool ONCE = false> __device__ __forceinline__ void load_lds16(const void* src, void* dst) {
+  __builtin_amdgcn_global_load_lds((glob_void*)src, (lds_void*)dst, 16, 0, ONCE ? 2 : 0);
 }
 
 // V operand of step s, dims 16 nb ..  16-bit types: ds_read_b64_tr_b16 gives lane i of each
@@ -499,16 +500,21 @@ __device__ __forceinline__ void store_part(const AttnP& a, const Row& r, int c, 
   *(f32x4*)(a.part + ((r.t * a.H + r.h) * a.nc + c) * HD + d) = o;
 }
 
+// (the largest instances would leave their lambdas as calls, their captures in scratch memory)
+#define ALTXS_INLINE __attribute__((always_inline))
+
 // ---- few rows ----------------------------------------------------------------
 //
-// Bound by the cache read.  64 segments decoding at 2048 keys of 8 x 64 bf16 (268 MB): 49 us,
-// 5.5 TB/s; 256 at 4096 (2.1 GB): 359 us, 6.0 TB/s (a large copy moves 5.1, a large read
+// Bound by the cache read.  64 segments decoding at 2048 keys of 8 x 64 bf16 (268 MB): 47 us,
+// 5.7 TB/s; 256 at 4096 (2.1 GB): 332 us, 6.5 TB/s (a large copy moves 5.1, a large read
 // 5.8).  A workgroup has its chunk's 64 KB in flight at once and a CU holds two of them, which
-// is what covers the memory latency; one segment at 2048 is all latency: 5.7 us in 64 workgroups of
-// a chunk each, and the fold's 3.8.
+// is what covers the memory latency; one segment at 2048 is all latency: 5.6 us in 64 workgroups of
+// a chunk each, and the fold's 3.8.  The loads are marked as read once: caches of several layers do
+// not stay in the memory-side cache from step to step (357 us without, and 49.3 / 47.5 over ten
+// caches of 64 segments, 34.6 / 31.6 of 32; caches that would stay, two of 32 segments, 29.2 / 31.1).
 
 template <class T, int HD, bool BIAS>
-__global__ __launch_bounds__(THREADS) void attn_few_kernel(AttnP a) {
+__global__ __launch_bounds__(THREADS, HD * sizeof(T) > 256 ? 1 : 2) void attn_few_kernel(AttnP a) {
 #pragma clang fp contract(off)
   constexpr int EL = Op<T>::EL, KS = HD / (4 * EL), ST = STEPS<T>;  // pieces of a score; steps of P V
   constexpr int NB = HD / 16 / WAVES;                              // 16-dim blocks of a wave's share of O
@@ -536,22 +542,34 @@ __global__ __launch_bounds__(THREADS) void attn_few_kernel(AttnP a) {
   for (int nb = 0; nb < NB; ++nb) O[nb] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int c_end = (seen.hi + CHUNK - 1) / CHUNK;
   if (seen.lo < seen.hi) {
-    for (int c = seen.lo / CHUNK + blockIdx.y; c < c_end; c += gridDim.y) {
-      const int k0 = c * CHUNK + wave * TILE;
-      const int pg = entry_page(a, key_entry(a, tile.b, k0 + lane, seen.lo, seen.hi), k0 + lane, seen.lo, seen.hi);
-      u32x4 k[4][KS];
+    // K of a chunk is loaded while the one before it goes through P V, and its page
+    // entries another chunk ahead (read for the nearest key of the union, past the end too).
+    u32x4 k[4][KS];
+    auto entry_of = [&](int64_t c) {
+      const int64_t key = c * CHUNK + wave * TILE + lane;
+      return key_entry(a, tile.b, key < seen.hi ? (int)key : seen.hi, seen.lo, seen.hi);
+    };
+    auto load_k = [&](int c, int entry) ALTXS_INLINE {
+      const int k0 = c * CHUNK + wave * TILE, pg = entry_page(a, entry, k0 + lane, seen.lo, seen.hi);
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb) {
         const int i = 16 * kb + col;
         const T* src = key_row<T>(a.k, __shfl(pg, i, WAVE), k0 + i, a.shift, a.kv_page, a.kv_slot, hk * a.kv_head);
 #pragma unroll
-        for (int s = 0; s < KS; ++s) k[kb][s] = *(const u32x4*)(src + EL * (4 * s + g));
+        for (int s = 0; s < KS; ++s) k[kb][s] = __builtin_nontemporal_load((const u32x4*)(src + EL * (4 * s + g)));
       }
+      return pg;
+    };
+    int c = seen.lo / CHUNK + blockIdx.y;
+    if (c >= c_end) return;  // (a shared row tile: the workgroup has no chunk of it)
+    int pg = load_k(c, entry_of(c)), entry = entry_of((int64_t)c + gridDim.y);
+    for (; c < c_end; c += gridDim.y) {
+      const int k0 = c * CHUNK + wave * TILE;
 #pragma unroll
       for (int i = 0; i < TILE / RPL; ++i) {
         const int vr = i * RPL + lane / PR;
         const T* src = key_row<T>(a.v, __shfl(pg, vr, WAVE), k0 + vr, a.shift, a.kv_page, a.kv_slot, hk * a.kv_head);
-        load_lds16(src + EL * v_piece<T, HD>(vr, lane % PR), vt[wave] + i * RPL * HD);
+        load_lds16<true>(src + EL * v_piece<T, HD>(vr, lane % PR), vt[wave] + i * RPL * HD);
       }
       f32x4 S[1][4];
 #pragma unroll
@@ -578,6 +596,10 @@ __global__ __launch_bounds__(THREADS) void attn_few_kernel(AttnP a) {
         if (lane == 0) odd[wave] = any;
       }
       __syncthreads();
+      if (c + (int)gridDim.y < c_end) {
+        pg = load_k(c + gridDim.y, entry);
+        entry = entry_of((int64_t)c + 2 * gridDim.y);
+      }
       f32x4 l[1] = {f32x4{0.f, 0.f, 0.f, 0.f}}, o[1][NB];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) o[0][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -652,9 +674,6 @@ __device__ __forceinline__ int many_slot(const AttnP& a, int i, int& hk) {
   hk = (int)div_by(pair, a.by_b);
   return (pair - hk * a.B + 1) * (int)a.by_tiles.d - 1 - back;
 }
-
-// (the largest instance would leave its lambdas as calls, their captures in scratch memory)
-#define ALTXS_INLINE __attribute__((always_inline))
 
 template <class T, int HD, bool BIAS>
 __global__ __launch_bounds__(NW* WAVE, HD * sizeof(T) > 256 ? 1 : 2) void attn_many_kernel(AttnP a) {
@@ -1008,21 +1027,27 @@ Plan plan_of(const AltxsPagedAttnArgs* a) {
   if (a->cu) tiles = std::max(std::min((int64_t)a->B, a->T), (a->T * G + br - 1) / br);
   tiles *= a->Hkv;
   // Share a row tile's chunks among workgroups where the row tiles alone do not fill the
-  // chip and the time that saves is well above the fold's: a launch, and the partial
-  // results written and read at ~3 TB/s.  A workgroup takes ~3.2 us a chunk (few) or
-  // ~4.8 (many).  Measured, one against shared: 2 segments decoding at 2048 22.6 / 9.4 us,
-  // 48 segments 42.3 / 43.6 (from 384 workgroups on they fill the chip); windows of 512
-  // tokens at 8000 163 / 37 us, but chunks of 1024 and 4096 tokens from position 0 24.2 / 23.5
-  // and 81 / 87.  Many rows share no further than one workgroup a place (2 x 256): 1024 took
-  // 40.4 for 37.3 of those windows; 48 drafts of up to 9 tokens 33.7 us counted by their slots and 31.0 by
-  // their tiles.
-  const int64_t fill = p.few ? 2048 : 512;
+  // chip and that saves well more than the fold costs: a launch, and the partial results
+  // written and read at ~3 TB/s.
+  // Few: a workgroup takes a chunk in 3.6 us (rows of 128 bytes) to 9.3 (of 512), half as
+  // long again where a CU holds two, and no call reads faster than ~6 TB/s.  Measured, one workgroup
+  // against shared: 2 segments decoding at 2048 22.6 / 9.4 us, 40 (8 heads of 64) 42.8 / 36.0, 48 42.3 /
+  // 43.6; 16 over 2 heads of 128 at 4096, 64 segments 85.7 / 58.1, 128 segments 97.3 / 114.6.
+  // Many: ~4.8 us a chunk.  Windows of 512 tokens at 8000 163 / 37 us, but chunks of 1024 and 4096
+  // tokens from position 0 24.2 / 23.5 and 81 / 87.
+  // Shared no further than what is resident: few 64 segments of 16 over 2 heads of 128 at 4096 58.1
+  // by 512 workgroups, 61.4 by 2048; many, those windows of 512 37.3 by 512, 40.4 by 1024; 48 drafts of up
+  // to 9 tokens 33.7 us counted by their slots and 31.0 by their tiles.
+  const int64_t fill = p.few ? 768 : 512;
   if (tiles < 384) {
     int64_t z = (fill + tiles - 1) / tiles;
     z = std::max<int64_t>(1, std::min<int64_t>({z, p.nc, 4 * fill / p.wgs}));  // idle segments' workgroups cost their start
-    const double chunk_us = p.few ? 3.2 : 4.8;
+    const int es = a->dtype == ALTXS_F32 ? 4 : 2;
     const double fold_us = 4.0 + (double)p.rows * p.nc * (a->head_dim + 2) * 8 / 3e6;
-    if (p.nc * chunk_us > 1.5 * ((p.nc + z - 1) / z * chunk_us + fold_us)) p.split = (int)z;
+    const double chunk_us = p.few ? (1.7 + 1.9 * a->head_dim * es / 128) * (tiles > 256 ? 1.5 : 1.0) : 4.8;
+    const double read_us = p.few ? (double)tiles * p.nc * CHUNK * a->head_dim * es * 2 / 6e6 : 0.0;
+    const double one = std::max(p.nc * chunk_us, read_us), shared = std::max((p.nc + z - 1) / z * chunk_us, read_us) + fold_us;
+    if (one > (p.few ? 1.15 : 1.5) * shared) p.split = (int)z;
   }
   return p;
 }
