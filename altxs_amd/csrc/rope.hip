@@ -11,7 +11,7 @@
 // that 16-byte accesses do not fit (strides, alignment, rot) go by units of one
 // pair or one element.
 //
-// Large calls are bound by memory: 65536 x 16 x 128 fp16 with its tables (571 MB) 115 us, 4.95
+// Large calls are bound by memory: 65536 x 16 x 128 fp16 with its tables (571 MB) 95 us, 6.0
 // TB/s (a large copy moves 5.1); 9973 x 8 x 64 fp32 (41 MB) 10.1 us; 16 segments' ragged chunks into
 // their pages (8 + 2 x 4 heads of 64 bf16, 60 MB) 18.7 us.  Small ones are a chain of latencies: 64 rows
 // 3.0 us, an append of 64 4.2 us (bounds, page entry, table row; the sources are read meanwhile).
@@ -26,6 +26,7 @@ namespace {
 using namespace altxs_paged;
 
 constexpr int THREADS = 256;
+constexpr double CACHE = 256 << 20;  // bytes of the memory-side cache
 
 template <class T> struct alignas(16) Vec { T v[16 / sizeof(T)]; };
 
@@ -40,6 +41,16 @@ template <class T> __device__ __forceinline__ T rounded(float x) {
   return (T)x;
 }
 
+// ONCE: what is not used again soon (the nt bit); 16-byte vectors only.
+template <bool ONCE, class V> __device__ __forceinline__ V load_as(const void* p) {
+  if constexpr (ONCE) return __builtin_bit_cast(V, __builtin_nontemporal_load((const u32x4*)p));
+  else return *(const V*)p;
+}
+template <bool ONCE, class V> __device__ __forceinline__ void store_as(void* p, const V& v) {
+  if constexpr (ONCE) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), (u32x4*)p);
+  else *(V*)p = v;
+}
+
 // How a head's row is cut into units.
 struct Units {
   int nrot;   // rotated units
@@ -50,7 +61,7 @@ struct Units {
 // One unit of one head row on its way: get() reads it, put() rotates and writes it.  A
 // kernel reads first and finds the position and the place meanwhile: both cost a
 // memory latency or three.  cs/sn: the position's table rows (NULL: copy).
-template <class T, bool VEC, bool INTER> struct Unit {
+template <class T, bool VEC, bool INTER, bool ONCE = false> struct Unit {
   static constexpr int N = VEC ? 16 / (int)sizeof(T) : 1;  // elements of a vector
   static constexpr bool PAIR = !VEC || !INTER;             // firsts and seconds are two accesses
   std::conditional_t<VEC, Vec<T>, T> x, y;
@@ -65,8 +76,8 @@ template <class T, bool VEC, bool INTER> struct Unit {
 
   __device__ __forceinline__ void get(const T* src, const Units& u) {
     using V = decltype(x);
-    x = *(const V*)(src + first(u));
-    if (PAIR && i < u.nrot) y = *(const V*)(src + second(u));
+    x = load_as<ONCE, V>(src + first(u));
+    if (PAIR && i < u.nrot) y = load_as<ONCE, V>(src + second(u));
   }
   __device__ __forceinline__ void put(const Units& u, float sgn) {
 #pragma clang fp contract(off)
@@ -98,8 +109,8 @@ template <class T, bool VEC, bool INTER> struct Unit {
         y = rounded<T>(__builtin_fmaf(-a, s, b * c));
       }
     }
-    *(V*)(dst + first(u)) = x;
-    if (PAIR && i < u.nrot) *(V*)(dst + second(u)) = y;
+    store_as<ONCE>(dst + first(u), x);
+    if (PAIR && i < u.nrot) store_as<ONCE>(dst + second(u), y);
   }
 };
 
@@ -117,7 +128,7 @@ struct RopeP {
   float sgn;
 };
 
-template <class T, bool VEC, bool INTER>
+template <class T, bool VEC, bool INTER, bool ONCE>
 __global__ __launch_bounds__(THREADS) void rope_kernel(RopeP p) {
   const int64_t t0 = (int64_t)blockIdx.x * p.tpb;
   const int nt = (int)(p.T - t0 < p.tpb ? p.T - t0 : p.tpb);
@@ -126,7 +137,7 @@ __global__ __launch_bounds__(THREADS) void rope_kernel(RopeP p) {
     const uint32_t tl = div_by(i, p.by_token), j = i - tl * p.by_token.d;
     const uint32_t h = div_by(j, p.by_units);
     const int64_t t = t0 + tl;
-    Unit<T, VEC, INTER> m;
+    Unit<T, VEC, INTER, ONCE> m;
     m.i = j - h * p.by_units.d;
     m.get((const T*)p.x + t * p.x_tok + h * p.x_head, p.u);
     const int32_t pos = p.pos[t];
@@ -242,19 +253,12 @@ Units units_of(int hd, int rot, bool vec, bool inter, int n) {
   return u;
 }
 
-#define BY_TYPE(KERNEL, dtype, vec, inter, grid, s, p)                                                    \
-  do {                                                                                                    \
-    auto go = [&](auto t) {                                                                               \
-      using T = decltype(t);                                                                              \
-      if (vec && inter) hipLaunchKernelGGL((KERNEL<T, true, true>), grid, dim3(THREADS), 0, s, p);        \
-      else if (vec) hipLaunchKernelGGL((KERNEL<T, true, false>), grid, dim3(THREADS), 0, s, p);           \
-      else if (inter) hipLaunchKernelGGL((KERNEL<T, false, true>), grid, dim3(THREADS), 0, s, p);         \
-      else hipLaunchKernelGGL((KERNEL<T, false, false>), grid, dim3(THREADS), 0, s, p);                   \
-    };                                                                                                    \
-    if (dtype == ALTXS_F32) go(float{});                                                                  \
-    else if (dtype == ALTXS_BF16) go(__bf16{});                                                           \
-    else go(_Float16{});                                                                                  \
-  } while (0)
+// f(T{}) for the type of dtype
+template <class F> void by_type(int dtype, F f) {
+  if (dtype == ALTXS_F32) f(float{});
+  else if (dtype == ALTXS_BF16) f(__bf16{});
+  else f(_Float16{});
+}
 
 }  // namespace
 
@@ -289,7 +293,19 @@ extern "C" int32_t altxs_rope(const AltxsRopeArgs* a, altxs_stream_t stream) {
   const int64_t wgs = (a->T + p.tpb - 1) / p.tpb;
   ALTXS_REQUIRE(wgs < (1ll << 24), "altxs_rope: T=%lld", (long long)a->T);  // 2^32 threads a launch
   const dim3 grid((unsigned)wgs);
-  BY_TYPE(rope_kernel, a->dtype, vec, inter, grid, (hipStream_t)stream, p);
+  // Arrays that together pass the memory-side cache leave little in it for who reads the
+  // result.  Marked as used once / not, two sets in turn: 536 MB 94.4 / 101 us, 268 MB 48.8 / 52.7, but 134 MB
+  // 25.9 / 25.2, and one set over and over, which stays, 268 MB 48.3 / 45.0.
+  const int es = elem_size(a->dtype);
+  const bool once = vec && 2.0 * (double)a->T * a->H * a->head_dim * es > CACHE;
+  by_type(a->dtype, [&](auto t) {
+    using T = decltype(t);
+    auto* k = !vec    ? inter ? rope_kernel<T, false, true, false> : rope_kernel<T, false, false, false>
+              : once  ? inter ? rope_kernel<T, true, true, true> : rope_kernel<T, true, false, true>
+              : inter ? rope_kernel<T, true, true, false>
+                      : rope_kernel<T, true, false, false>;
+    hipLaunchKernelGGL(k, grid, dim3(THREADS), 0, (hipStream_t)stream, p);
+  });
   ALTXS_CHECK_HIP(hipGetLastError());
   return ALTXS_OK;
 }
@@ -346,7 +362,12 @@ extern "C" int32_t altxs_paged_append(const AltxsPagedAppendArgs* a, altxs_strea
   const int64_t wgs = (a->T + p.tpb - 1) / p.tpb;
   ALTXS_REQUIRE(wgs < (1ll << 24), "altxs_paged_append: T=%lld", (long long)a->T);
   const dim3 grid((unsigned)wgs);
-  BY_TYPE(append_kernel, a->dtype, vec, inter, grid, (hipStream_t)stream, p);
+  by_type(a->dtype, [&](auto t) {
+    using T = decltype(t);
+    auto* k = vec ? inter ? append_kernel<T, true, true> : append_kernel<T, true, false>
+                  : inter ? append_kernel<T, false, true> : append_kernel<T, false, false>;
+    hipLaunchKernelGGL(k, grid, dim3(THREADS), 0, (hipStream_t)stream, p);
+  });
   ALTXS_CHECK_HIP(hipGetLastError());
   return ALTXS_OK;
 }

@@ -144,6 +144,26 @@ def test_rope_far_positions_and_long_arrays():
     assert torch.equal(x[T - 5 - (T - 5) % 64:], x[:T - (T - 5 - (T - 5) % 64)])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_of_arrays_past_the_cache(dtype, interleaved):
+    """Arrays of more than 256 MB are loaded and stored otherwise: the bits of its parts."""
+    from altxs_amd import ops
+
+    T, H, hd, part = 40001, 16, 128, 9000
+    _log(f"rope of a large array {dtype} interleaved={interleaved}")
+    cos, sin = _tables(500, 64)
+    g = torch.Generator(device=DEV).manual_seed(11)
+    x = torch.randn(T, H, hd, generator=g, device=DEV, dtype=torch.float32).to(dtype)
+    assert 2 * x.numel() * x.element_size() > 256 << 20 > 2 * part * H * hd * x.element_size()
+    pos = torch.randint(-1, 500, (T,), generator=g, device=DEV, dtype=torch.int32)
+    got = ops.rope(x, pos, cos, sin, interleaved=interleaved)
+    for t in range(0, T, part):
+        want = ops.rope(x[t:t + part], pos[t:t + part], cos, sin, interleaved=interleaved)
+        assert torch.equal(_bits(got[t:t + part]), _bits(want))
+    assert ops.rope(x, pos, cos, sin, interleaved=interleaved, out=x) is x and torch.equal(_bits(x), _bits(got))
+
+
 def test_rope_refuses():
     from altxs_amd import ops
 
