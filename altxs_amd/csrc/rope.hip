@@ -11,9 +11,9 @@
 // that 16-byte accesses do not fit (strides, alignment, rot) go by units of one
 // pair or one element.
 //
-// Large calls are bound by memory: 65536 x 16 x 128 fp16 with its tables (571 MB) 95 us, 6.0
-// TB/s (a large copy moves 5.1); 9973 x 8 x 64 fp32 (41 MB) 10.1 us; 16 segments' ragged chunks into
-// their pages (8 + 2 x 4 heads of 64 bf16, 60 MB) 18.7 us.  Small ones are a chain of latencies: 64 rows
+// Large calls are bound by memory: 65536 x 16 x 128 fp16 with its tables (571 MB) 92.5 us, 6.2
+// TB/s (a large copy moves 5.1); 9973 x 8 x 64 fp32 (41 MB) 9.8 us; 16 segments' ragged chunks into
+// their pages (8 + 2 x 4 heads of 64 bf16, 60 MB) 18.4 us.  Small ones are a chain of latencies: 64 rows
 // 3.0 us, an append of 64 4.2 us (bounds, page entry, table row; the sources are read meanwhile).
 // Four units a thread instead of one changed nothing.
 #include <type_traits>
