@@ -454,8 +454,9 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
                starts: torch.Tensor | None = None, prefix: torch.Tensor | None = None,
                out: torch.Tensor | None = None, err: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of the new tokens q [T, H, hd] (hd 64 or 128; fp32, bf16 or fp16; rows
-    of q and the caches at multiples of 16 bytes) over their segments' pages, in which their own keys and values already are (:func:`paged_append`
-    with the same table, pos and cu); H a multiple of the cache's heads.
+    of q and the caches at multiples of 16 bytes) over their segments' pages, in which
+    their own keys and values already are (:func:`paged_append` with the same table, pos
+    and cu); H a multiple of the cache's heads.
 
     The token at position p sees the keys [lo, hi): hi = p + 1, or the first
     ``prefix[b]`` keys of the segment if that is more (int32 [B]; a prefix mask);
@@ -465,7 +466,7 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
     ``slopes[h]`` (fp32 [H]) * |p - key|.  A token that sees nothing gets zeros; rows
     behind the last segment keep what ``out`` held.
 
-    ``max_len``: the most keys any segment has (default: what its table can
+    ``max_len``: the most keys any segment has (at most 2^30; default: what its table can
     hold); it sizes the launch, so give it where it is known.  A row's bits
     depend on the row's own query, keys and masks alone.
     """
